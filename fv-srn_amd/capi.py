@@ -69,6 +69,18 @@ PREINTEGRATE_NONE, PREINTEGRATE_1D, PREINTEGRATE_2D = 0, 1, 2
 TF_GAUSSIAN_PLAIN, TF_GAUSSIAN_SCALE_WITH_GRADIENT, TF_GAUSSIAN_ANALYTIC = 0, 1, 2
 
 
+class ScanDesc(C.Structure):
+    _fields_ = [("dtype", C.c_int), ("gate_mode", C.c_int), ("input_mode", C.c_int), ("reverse", C.c_int), ("gate_scale", C.c_float),
+                ("length", C.c_int), ("batch", C.c_longlong), ("channels", C.c_longlong), ("gate_channels", C.c_longlong),
+                ("gate_stride", C.c_longlong * 3), ("x_stride", C.c_longlong * 3), ("out_stride", C.c_longlong * 3),
+                ("dout_stride", C.c_longlong * 3), ("dgate_stride", C.c_longlong * 3), ("dx_stride", C.c_longlong * 3)]
+
+
+GATE_VALUE, GATE_EXP = 0, 1
+INPUT_ADD, INPUT_BLEND = 0, 1
+_TENSOR_DTYPES = {"torch.float32": 0, "torch.float16": 1, "torch.bfloat16": 2}
+
+
 # every symbol include/fvsrn.h declares: (name, restype, argtypes)
 _VP, _SZ, _I, _F, _D = C.c_void_p, C.c_size_t, C.c_int, C.c_float, C.c_double
 _FP, _DP, _U16P = C.POINTER(C.c_float), C.POINTER(C.c_double), C.POINTER(C.c_uint16)
@@ -134,6 +146,12 @@ SYMBOLS = [
     ("fvsrn_cvol_read", _I, [C.c_char_p, _FP, _VP, _VP]),
     ("fvsrn_volume_evaluate_points", _I, [_VP, _I, _I, _I, _VP, _SZ, _VP, _VP]),
     ("fvsrn_render_volume", _I, [_VP, _VP, _I, _I, _I, _I, _I, _I, _VP, _VP, _VP]),
+    ("fvsrn_quantize_rows", _I, [_VP, _I, C.c_longlong, _I, C.c_longlong, _VP, C.c_longlong, _VP, _VP]),
+    ("fvsrn_matmul_int8", _I, [_VP, C.c_longlong, _VP, _VP, C.c_longlong, _VP, _VP, C.c_longlong, _I, _I, _I, _F, _VP, _I, C.c_longlong, _VP]),
+    ("fvsrn_scan_desc_size", _SZ, []),
+    ("fvsrn_gated_scan_workspace", _I, [C.POINTER(ScanDesc), _I, C.POINTER(_SZ)]),
+    ("fvsrn_gated_scan", _I, [C.POINTER(ScanDesc), _VP, _VP, _VP, _VP, _VP, _VP, _VP, _SZ, _VP]),
+    ("fvsrn_gated_scan_backward", _I, [C.POINTER(ScanDesc), _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _SZ, _VP]),
 ]
 
 _lib = None
@@ -161,6 +179,8 @@ def lib() -> C.CDLL:
             fn.restype = res
             fn.argtypes = args
         if l.fvsrn_scene_desc_size() != C.sizeof(SceneDesc) or l.fvsrn_network_info_size() != C.sizeof(NetworkInfo):
+            raise FvsrnError(-1, "capi.py struct mirrors do not match include/fvsrn.h of the loaded libfvsrn.so")
+        if hasattr(l, "fvsrn_scan_desc_size") and l.fvsrn_scan_desc_size() != C.sizeof(ScanDesc):
             raise FvsrnError(-1, "capi.py struct mirrors do not match include/fvsrn.h of the loaded libfvsrn.so")
         _lib = l
     return _lib
@@ -706,3 +726,180 @@ def generate_rays(eye, right, up, fov_y_radians: float, width: int, height: int,
     s = torch.cuda.current_stream().cuda_stream if stream is None else stream
     _check(lib().fvsrn_generate_rays(_fptr(e), _fptr(r), _fptr(u), fov_y_radians, width, height, start.data_ptr(), direction.data_ptr(), s))
     return start, direction
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# Tensor operators of a ray march in pieces (include/fvsrn.h: fvsrn_quantize_rows, fvsrn_matmul_int8, fvsrn_gated_scan, fvsrn_gated_scan_backward)
+# ---------------------------------------------------------------------------------------------------------------------
+
+def _operand(t, what: str, dtype=None, shape=None):
+    """A tensor of the current device, of the given dtype and shape, whatever its strides."""
+    import torch
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise FvsrnError(-1, "%s must be a CUDA(HIP) tensor" % what)
+    if t.device.index != torch.cuda.current_device():
+        raise FvsrnError(ERR_WRONG_DEVICE, "%s is on HIP device %d, but the current device is %d" % (what, t.device.index, torch.cuda.current_device()))
+    if dtype is not None and t.dtype != dtype:
+        raise FvsrnError(-1, "%s must be %s" % (what, dtype))
+    if shape is not None and tuple(t.shape) != tuple(shape):
+        raise FvsrnError(-1, "%s must be of shape %s, not %s" % (what, tuple(shape), tuple(t.shape)))
+    return t
+
+
+def _dense(t, what: str, dtype, shape):
+    _operand(t, what, dtype, shape)
+    if not t.is_contiguous():
+        raise FvsrnError(-1, "%s must be contiguous" % what)
+    return t
+
+
+def _rows(t, what: str, dtype=None):
+    """A matrix whose rows are contiguous; its row stride."""
+    _operand(t, what, dtype)
+    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
+        raise FvsrnError(-1, "%s must be a matrix with contiguous rows" % what)
+    return t.stride(0)
+
+
+class _OnStream:
+    """Allocations of a call belong to the stream it runs on: `stream` (a raw handle) or torch's current one."""
+
+    def __init__(self, stream):
+        import torch
+        current = torch.cuda.current_stream().cuda_stream
+        self.handle = current if stream is None else stream
+        self._other = torch.cuda.stream(torch.cuda.ExternalStream(self.handle)) if self.handle != current else None
+
+    def __enter__(self):
+        if self._other is not None:
+            self._other.__enter__()
+        return self.handle
+
+    def __exit__(self, *a):
+        if self._other is not None:
+            self._other.__exit__(*a)
+
+
+def quantize_rows(x, codes=None, scales=None, stream: Optional[int] = None):
+    """Codes (rows, cols) int8 and scales (rows,) float32 of the rows of a float32 / float16 / bfloat16 matrix (fvsrn_quantize_rows): scale = max |x| / 127, code =
+    x / scale to the nearest.  Tokens and the (out, in) weights of a layer alike.  A row that holds an infinity or a NaN: scale NaN, codes 0."""
+    import torch
+    ldx = _rows(x, "x")
+    if str(x.dtype) not in _TENSOR_DTYPES:
+        raise FvsrnError(-1, "x must be float32, float16 or bfloat16")
+    with _OnStream(stream) as s:
+        if codes is None:
+            codes = torch.empty(x.shape, dtype=torch.int8, device=x.device)
+        if scales is None:
+            scales = torch.empty(x.shape[0], dtype=torch.float32, device=x.device)
+        ldc = _rows(_operand(codes, "codes", torch.int8, x.shape), "codes")
+        _dense(scales, "scales", torch.float32, (x.shape[0],))
+        _check(lib().fvsrn_quantize_rows(x.data_ptr(), _TENSOR_DTYPES[str(x.dtype)], x.shape[0], x.shape[1], ldx, codes.data_ptr(), ldc, scales.data_ptr(), s))
+    return codes, scales
+
+
+def matmul_int8(a, scale_a, b, scale_b, bias=None, activation: str = "None", activation_param: float = 1.0, dtype=None, out=None, stream: Optional[int] = None):
+    """A layer in 8-bit integers (fvsrn_matmul_int8): act((a b^T) scale_a scale_b + bias), a (M, K) int8 tokens with scale_a (M,), b (N, K) int8 weights with
+    scale_b (N,) (both of quantize_rows), bias (N,) float32 or None, activation one of ACTIVATIONS.  out: (M, N) of `dtype` (float32)."""
+    import torch
+    lda, ldb = _rows(a, "a", torch.int8), _rows(b, "b", torch.int8)
+    M, K, N = a.shape[0], a.shape[1], b.shape[0]
+    if b.shape[1] != K:
+        raise FvsrnError(-1, "a and b must have rows of the same length")
+    _dense(scale_a, "scale_a", torch.float32, (M,))
+    _dense(scale_b, "scale_b", torch.float32, (N,))
+    if bias is not None:
+        _dense(bias, "bias", torch.float32, (N,))
+    if activation not in ACTIVATIONS:
+        raise FvsrnError(-1, "unknown activation %r" % (activation,))
+    if dtype is None:
+        dtype = torch.float32 if out is None else out.dtype
+    if str(dtype) not in _TENSOR_DTYPES:
+        raise FvsrnError(-1, "the output must be float32, float16 or bfloat16")
+    with _OnStream(stream) as s:
+        if out is None:
+            out = torch.empty((M, N), dtype=dtype, device=a.device)
+        ldo = _rows(_operand(out, "out", dtype, (M, N)), "out")
+        _check(lib().fvsrn_matmul_int8(a.data_ptr(), lda, scale_a.data_ptr(), b.data_ptr(), ldb, scale_b.data_ptr(), None if bias is None else bias.data_ptr(), M, N, K,
+                                       ACTIVATIONS[activation], float(activation_param), out.data_ptr(), _TENSOR_DTYPES[str(dtype)], ldo, s))
+    return out
+
+
+def _scan_desc(gate, x, gate_mode, gate_scale, input_mode, reverse, h0, lengths):
+    import torch
+    _operand(gate, "gate")
+    if str(gate.dtype) not in _TENSOR_DTYPES:
+        raise FvsrnError(-1, "gate must be float32, float16 or bfloat16")
+    _operand(x, "x", gate.dtype)
+    if gate.dim() != 3 or x.dim() != 3 or gate.shape[:2] != x.shape[:2]:
+        raise FvsrnError(-1, "gate must be (batch, steps, gate channels) and x (batch, steps, channels)")
+    d = ScanDesc()
+    d.dtype, d.gate_mode, d.input_mode, d.reverse, d.gate_scale = _TENSOR_DTYPES[str(gate.dtype)], gate_mode, input_mode, int(reverse), gate_scale
+    d.batch, d.length, d.channels, d.gate_channels = x.shape[0], x.shape[1], x.shape[2], gate.shape[2]
+    d.gate_stride[:], d.x_stride[:] = gate.stride(), x.stride()
+    if h0 is not None:
+        _dense(h0, "h0", torch.float32, (x.shape[0], x.shape[2]))
+    if lengths is not None:
+        _dense(lengths, "lengths", torch.int32, (x.shape[0],))
+    return d
+
+
+def _scan_workspace(d, backward, device):
+    import torch
+    n = _SZ(0)
+    _check(lib().fvsrn_gated_scan_workspace(C.byref(d), backward, C.byref(n)))
+    return (torch.empty(n.value, dtype=torch.uint8, device=device) if n.value else None), n.value
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def gated_scan(gate, x, *, gate_mode: int = GATE_VALUE, gate_scale: float = 1.0, input_mode: int = INPUT_ADD, reverse: bool = False, h0=None, lengths=None,
+               states: bool = True, out=None, last=None, stream: Optional[int] = None):
+    """h_t = a_t h_{t-1} + u_t over (batch, steps, channels), a_t = gate or exp(gate_scale * gate), u_t = x or (1 - a_t) x (fvsrn_gated_scan).  gate has (batch,
+    steps, gate channels), each for channels / gate channels adjacent channels of x.  Returns (all states -- None with states=False --, the last state (batch,
+    channels) float32).  h0: float32 (batch, channels); lengths: int32 (batch,); last may be h0: a march that steps in place.
+
+    Beer-Lambert blending of the colours (rays, samples, rgb + absorption) that Scene.evaluate_tf gives, back to front:
+        _, rgb = gated_scan(c[..., 3:], c[..., :3], gate_mode=GATE_EXP, gate_scale=-stepsize, input_mode=INPUT_BLEND, reverse=True, states=False)"""
+    import torch
+    d = _scan_desc(gate, x, gate_mode, gate_scale, input_mode, reverse, h0, lengths)
+    with _OnStream(stream) as s:
+        if out is None and states:
+            out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        if last is None:
+            last = torch.empty((x.shape[0], x.shape[2]), dtype=torch.float32, device=x.device)
+        _dense(last, "last", torch.float32, (x.shape[0], x.shape[2]))
+        if out is not None:
+            d.out_stride[:] = _operand(out, "out", x.dtype, x.shape).stride()
+        ws, n = _scan_workspace(d, 0, x.device)
+        _check(lib().fvsrn_gated_scan(C.byref(d), gate.data_ptr(), x.data_ptr(), _ptr(h0), _ptr(lengths), _ptr(out), last.data_ptr(), _ptr(ws), n, s))
+    return out, last
+
+
+def gated_scan_backward(gate, x, dout=None, dlast=None, *, gate_mode: int = GATE_VALUE, gate_scale: float = 1.0, input_mode: int = INPUT_ADD, reverse: bool = False,
+                        h0=None, lengths=None, dgate=None, dx=None, dh0=None, stream: Optional[int] = None):
+    """Gradients (dgate, dx, dh0) of gated_scan with the same arguments for dout (of the states) and / or dlast (of the last state, float32); dh0 is None without
+    h0 (fvsrn_gated_scan_backward).  Inputs that were broadcast (expand) get their gradient per element."""
+    import torch
+    d = _scan_desc(gate, x, gate_mode, gate_scale, input_mode, reverse, h0, lengths)
+    if dout is not None:
+        d.dout_stride[:] = _operand(dout, "dout", x.dtype, x.shape).stride()
+    if dlast is not None:
+        _dense(dlast, "dlast", torch.float32, (x.shape[0], x.shape[2]))
+    with _OnStream(stream) as s:
+        if dgate is None:
+            dgate = torch.empty(gate.shape, dtype=gate.dtype, device=gate.device)
+        if dx is None:
+            dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        if dh0 is None and h0 is not None:
+            dh0 = torch.empty_like(h0)
+        if dh0 is not None:
+            _dense(dh0, "dh0", torch.float32, (x.shape[0], x.shape[2]))
+        d.dgate_stride[:] = _operand(dgate, "dgate", gate.dtype, gate.shape).stride()
+        d.dx_stride[:] = _operand(dx, "dx", x.dtype, x.shape).stride()
+        ws, n = _scan_workspace(d, 1, x.device)
+        _check(lib().fvsrn_gated_scan_backward(C.byref(d), gate.data_ptr(), x.data_ptr(), _ptr(h0), _ptr(lengths), _ptr(dout), _ptr(dlast), dgate.data_ptr(),
+                                               dx.data_ptr(), _ptr(dh0), _ptr(ws), n, s))
+    return dgate, dx, dh0

@@ -482,6 +482,69 @@ int fvsrn_volume_evaluate_points(fvsrn_volume* volume, int source, int interpola
 int fvsrn_render_volume(fvsrn_scene* scene, fvsrn_volume* volume, int source, int interpolation, int grid_resolution_new_behavior,
                         int provide_normals, int width, int height, float* d_out8, unsigned long long* d_stats, void* stream);
 
+/* ---------------------------------------------------------------------------------------------------------------------
+ * Tensor operators of a ray march in pieces: rays (fvsrn_generate_rays), network at the samples (fvsrn_evaluate_points), colours
+ * (fvsrn_scene_evaluate_tf) -- and, below, layers wider than the fused kernels hold (8-bit) and the blend along the ray with its
+ * gradients.  No reference counterpart.
+ *
+ * Conventions on top of those at the head of this file: all pointers are device pointers of the current device; strides and sizes are in
+ * elements; the calls allocate nothing (where one needs scratch memory the caller hands it in), read no device memory on the host and may
+ * be captured into a graph.  Outputs must not overlap inputs or each other (FVSRN_ERR_INVALID_ARGUMENT where their address ranges do),
+ * except where an entry says so.  A size of zero is a call that does nothing more than its definition says (no rows: nothing). */
+typedef enum { FVSRN_TENSOR_F32 = 0, FVSRN_TENSOR_F16 = 1, FVSRN_TENSOR_BF16 = 2 } fvsrn_tensor_dtype;
+
+/* Codes and scales of the rows of a matrix x [rows][cols] (row stride ldx): scale = max(max_k |x_k| / 127, 2^-126), code = x / scale rounded
+ * to the nearest integer, ties to even; quotients are rounded to 32 bits.  A row that holds an infinity or a NaN gets the scale NaN and codes 0, so
+ * that every product with it is NaN.  For tokens (the rows of an activation matrix) and for the channels of a layer (the rows of its
+ * [out][in] weights) alike.  d_codes [rows][cols] with row stride ldc, d_scales [rows]. */
+int fvsrn_quantize_rows(const void* d_x, int dtype, long long rows, int cols, long long ldx, signed char* d_codes, long long ldc,
+                        float* d_scales, void* stream);
+
+/* A layer in 8-bit integers: out[m][n] = act((sum_k a[m][k] b[n][k]) * scale_b[n] * scale_a[m] + bias[n]) with a [M][K] (tokens), b [N][K]
+ * (weights, one row per output channel).  The sum is exact (32-bit integers, 1 <= K <= 131071), everything behind it is in 32-bit floats and is
+ * rounded once to out_dtype (fvsrn_tensor_dtype).  d_bias may be NULL; activation is an fvsrn_activation with its parameter as in
+ * fvsrn_network_add_layer (read by Sine, Snake and SnakeAlt; not 0 there).  Any alignment and row stride; rows of 16-byte aligned
+ * addresses and strides are the fast path. */
+int fvsrn_matmul_int8(const signed char* d_a, long long lda, const float* d_scale_a, const signed char* d_b, long long ldb, const float* d_scale_b,
+                      const float* d_bias, long long M, int N, int K, int activation, float act_param, void* d_out, int out_dtype, long long ldo,
+                      void* stream);
+
+/* The gated linear recurrence h_t = a_t h_{t-1} + u_t over a batch of sequences, each channel on its own:
+ *   a_t = gate_t (FVSRN_GATE_VALUE) or exp(gate_scale * gate_t) (FVSRN_GATE_EXP),
+ *   u_t = x_t (FVSRN_INPUT_ADD) or (1 - a_t) x_t (FVSRN_INPUT_BLEND),   h_{-1} = h0 or 0,
+ * with t running forwards or (reverse) backwards.  Channel c goes by gate c / (channels / gate_channels).  Beer-Lambert blending of n samples
+ * along a ray is EXP with gate = absorption and gate_scale = -stepsize, alpha blending is VALUE with gate = 1 - alpha; both BLEND and reverse
+ * (back to front), the pixel is `last`.  Gates may be any numbers; products of gates are formed over spans of a sequence, so gates
+ * of a magnitude over 1 can overflow there although the recurrence itself would not.
+ * d_lengths (int32 per batch element, clamped to 0 .. length; NULL: all `length`): behind a sequence's length nothing is read, and outputs and
+ * gradients there are written as zero.  The state is held in 32 bits whatever the dtype; h0 and last are [batch][channels] floats.
+ * Inputs may have any strides, zero and negative ones too (broadcast inputs; their gradients come per element); outputs may not overlap themselves. */
+typedef enum { FVSRN_GATE_VALUE = 0, FVSRN_GATE_EXP = 1 } fvsrn_gate_mode;
+typedef enum { FVSRN_INPUT_ADD = 0, FVSRN_INPUT_BLEND = 1 } fvsrn_input_mode;
+typedef struct {
+    int dtype;                        /* fvsrn_tensor_dtype of gate, x, out and of dout, dgate, dx                      */
+    int gate_mode, input_mode;        /* fvsrn_gate_mode, fvsrn_input_mode                                              */
+    int reverse;
+    float gate_scale;                 /* FVSRN_GATE_EXP                                                                 */
+    int length;                       /* steps T                                                                        */
+    long long batch, channels, gate_channels; /* gate_channels divides channels                                         */
+    long long gate_stride[3], x_stride[3];    /* batch, step, channel; gate is [batch][T][gate_channels], x [batch][T][channels] */
+    long long out_stride[3];          /* states, and ignored without them                                               */
+    long long dout_stride[3], dgate_stride[3], dx_stride[3]; /* backward only                                           */
+} fvsrn_scan_desc;
+size_t fvsrn_scan_desc_size(void);
+/* bytes of scratch memory that the call (backward != 0: the backward one) needs for this description; 0 is possible */
+int fvsrn_gated_scan_workspace(const fvsrn_scan_desc* desc, int backward, size_t* bytes);
+/* d_out (all states) and d_last (the last ones) may each be NULL; d_last may be d_h0 (a march that steps in place). */
+int fvsrn_gated_scan(const fvsrn_scan_desc* desc, const void* d_gate, const void* d_x, const float* d_h0, const int* d_lengths, void* d_out,
+                     float* d_last, void* d_workspace, size_t workspace_bytes, void* stream);
+/* Gradients for d_dout (of the states; NULL: none) and d_dlast (of `last`; NULL: none): d_dgate [batch][T][gate_channels] (summed over the channels of a
+ * gate), d_dx [batch][T][channels], d_dh0 [batch][channels]; each may be NULL.  The states are computed again in 32 bits.  Sums have a fixed
+ * order: the same call gives the same bits. */
+int fvsrn_gated_scan_backward(const fvsrn_scan_desc* desc, const void* d_gate, const void* d_x, const float* d_h0, const int* d_lengths,
+                              const void* d_dout, const float* d_dlast, void* d_dgate, void* d_dx, float* d_dh0, void* d_workspace,
+                              size_t workspace_bytes, void* stream);
+
 /* Kernel name of the variant fvsrn_render / fvsrn_evaluate_points would launch for this network: writes a 0-terminated string.
  * For renders this is a forecast from the network alone -- a latent grid is reported with the cell-table kernel whenever a table exists,
  * "(cells or gathers by footprint)" marks the automatic mode; the launch's own choice is fvsrn_scene_last_kernel_name. */
