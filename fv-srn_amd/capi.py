@@ -8,6 +8,7 @@ if the library or a GPU is missing the calls raise.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import os
 from typing import Optional, Sequence
 
@@ -78,7 +79,6 @@ class ScanDesc(C.Structure):
 
 GATE_VALUE, GATE_EXP = 0, 1
 INPUT_ADD, INPUT_BLEND = 0, 1
-_TENSOR_DTYPES = {"torch.float32": 0, "torch.float16": 1, "torch.bfloat16": 2}
 
 
 # every symbol include/fvsrn.h declares: (name, restype, argtypes)
@@ -732,69 +732,87 @@ def generate_rays(eye, right, up, fov_y_radians: float, width: int, height: int,
 # Tensor operators of a ray march in pieces (include/fvsrn.h: fvsrn_quantize_rows, fvsrn_matmul_int8, fvsrn_gated_scan, fvsrn_gated_scan_backward)
 # ---------------------------------------------------------------------------------------------------------------------
 
-def _operand(t, what: str, dtype=None, shape=None):
-    """A tensor of the current device, of the given dtype and shape, whatever its strides."""
+# A step of a march is a call of a few microseconds: what these bindings look up is looked up once (the dtype codes) or kept by shape (descriptions of scans).
+
+@functools.lru_cache(maxsize=None)
+def _tensor_dtypes():
     import torch
-    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+    return {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+
+
+def _refuse_device(t, what: str, device: int):
+    if t is None or not hasattr(t, "is_cuda") or not t.is_cuda:
         raise FvsrnError(-1, "%s must be a CUDA(HIP) tensor" % what)
-    if t.device.index != torch.cuda.current_device():
-        raise FvsrnError(ERR_WRONG_DEVICE, "%s is on HIP device %d, but the current device is %d" % (what, t.device.index, torch.cuda.current_device()))
-    if dtype is not None and t.dtype != dtype:
+    raise FvsrnError(ERR_WRONG_DEVICE, "%s is on HIP device %d, but the current device is %d" % (what, t.get_device(), device))
+
+
+def _operand(t, what: str, device: int, dtype, shape=None) -> int:
+    """The address of a tensor of the current device, of the given dtype and shape, whatever its strides."""
+    if not hasattr(t, "get_device") or not t.is_cuda or t.get_device() != device:
+        _refuse_device(t, what, device)
+    if t.dtype != dtype:
         raise FvsrnError(-1, "%s must be %s" % (what, dtype))
-    if shape is not None and tuple(t.shape) != tuple(shape):
+    if shape is not None and t.shape != shape:
         raise FvsrnError(-1, "%s must be of shape %s, not %s" % (what, tuple(shape), tuple(t.shape)))
-    return t
+    return t.data_ptr()
 
 
-def _dense(t, what: str, dtype, shape):
-    _operand(t, what, dtype, shape)
+def _dense(t, what: str, device: int, dtype, shape) -> int:
+    p = _operand(t, what, device, dtype, shape)
     if not t.is_contiguous():
         raise FvsrnError(-1, "%s must be contiguous" % what)
-    return t
+    return p
 
 
-def _rows(t, what: str, dtype=None):
-    """A matrix whose rows are contiguous; its row stride."""
-    _operand(t, what, dtype)
-    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
+def _row_stride(t, what: str) -> int:
+    """The row stride of a matrix whose rows are contiguous."""
+    if t.dim() != 2 or (t.stride(1) != 1 and t.shape[1] > 1):
         raise FvsrnError(-1, "%s must be a matrix with contiguous rows" % what)
     return t.stride(0)
 
 
-class _OnStream:
-    """Allocations of a call belong to the stream it runs on: `stream` (a raw handle) or torch's current one."""
+def _launch_state(t, what: str, stream):
+    """(the current device, the handle of the stream of a call -- `stream` or torch's current one --, a context for its allocations or None where they
+    belong to the current stream anyway); t: the first operand, without a device there is nothing to ask"""
+    import torch
+    if not getattr(t, "is_cuda", False):
+        _refuse_device(t, what, -1)
+    device = torch.cuda.current_device()
+    current = _raw_stream()(device)
+    if stream is None or stream == current:
+        return device, current, None
+    return device, stream, torch.cuda.stream(torch.cuda.ExternalStream(stream))
 
-    def __init__(self, stream):
-        import torch
-        current = torch.cuda.current_stream().cuda_stream
-        self.handle = current if stream is None else stream
-        self._other = torch.cuda.stream(torch.cuda.ExternalStream(self.handle)) if self.handle != current else None
 
-    def __enter__(self):
-        if self._other is not None:
-            self._other.__enter__()
-        return self.handle
+@functools.lru_cache(maxsize=None)
+def _raw_stream():
+    import torch
+    return getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda device: torch.cuda.current_stream(device).cuda_stream)
 
-    def __exit__(self, *a):
-        if self._other is not None:
-            self._other.__exit__(*a)
+
+def _allocated(context, make):
+    if context is None:
+        return make()
+    with context:
+        return make()
 
 
 def quantize_rows(x, codes=None, scales=None, stream: Optional[int] = None):
     """Codes (rows, cols) int8 and scales (rows,) float32 of the rows of a float32 / float16 / bfloat16 matrix (fvsrn_quantize_rows): scale = max |x| / 127, code =
     x / scale to the nearest.  Tokens and the (out, in) weights of a layer alike.  A row that holds an infinity or a NaN: scale NaN, codes 0."""
     import torch
-    ldx = _rows(x, "x")
-    if str(x.dtype) not in _TENSOR_DTYPES:
+    device, s, context = _launch_state(x, "x", stream)
+    code = _tensor_dtypes().get(getattr(x, "dtype", None))
+    if code is None:
         raise FvsrnError(-1, "x must be float32, float16 or bfloat16")
-    with _OnStream(stream) as s:
-        if codes is None:
-            codes = torch.empty(x.shape, dtype=torch.int8, device=x.device)
-        if scales is None:
-            scales = torch.empty(x.shape[0], dtype=torch.float32, device=x.device)
-        ldc = _rows(_operand(codes, "codes", torch.int8, x.shape), "codes")
-        _dense(scales, "scales", torch.float32, (x.shape[0],))
-        _check(lib().fvsrn_quantize_rows(x.data_ptr(), _TENSOR_DTYPES[str(x.dtype)], x.shape[0], x.shape[1], ldx, codes.data_ptr(), ldc, scales.data_ptr(), s))
+    xp = _operand(x, "x", device, x.dtype)
+    ldx, (rows, cols) = _row_stride(x, "x"), x.shape
+    if codes is None:
+        codes = _allocated(context, lambda: torch.empty((rows, cols), dtype=torch.int8, device=x.device))
+    if scales is None:
+        scales = _allocated(context, lambda: torch.empty(rows, dtype=torch.float32, device=x.device))
+    qp, sp = _operand(codes, "codes", device, torch.int8, x.shape), _dense(scales, "scales", device, torch.float32, (rows,))
+    _check(lib().fvsrn_quantize_rows(xp, code, rows, cols, ldx, qp, _row_stride(codes, "codes"), sp, s))
     return codes, scales
 
 
@@ -802,57 +820,43 @@ def matmul_int8(a, scale_a, b, scale_b, bias=None, activation: str = "None", act
     """A layer in 8-bit integers (fvsrn_matmul_int8): act((a b^T) scale_a scale_b + bias), a (M, K) int8 tokens with scale_a (M,), b (N, K) int8 weights with
     scale_b (N,) (both of quantize_rows), bias (N,) float32 or None, activation one of ACTIVATIONS.  out: (M, N) of `dtype` (float32)."""
     import torch
-    lda, ldb = _rows(a, "a", torch.int8), _rows(b, "b", torch.int8)
-    M, K, N = a.shape[0], a.shape[1], b.shape[0]
-    if b.shape[1] != K:
+    device, s, context = _launch_state(a, "a", stream)
+    ap, bp = _operand(a, "a", device, torch.int8), _operand(b, "b", device, torch.int8)
+    lda, ldb = _row_stride(a, "a"), _row_stride(b, "b")
+    (M, K), (N, Kb) = a.shape, b.shape
+    if Kb != K:
         raise FvsrnError(-1, "a and b must have rows of the same length")
-    _dense(scale_a, "scale_a", torch.float32, (M,))
-    _dense(scale_b, "scale_b", torch.float32, (N,))
-    if bias is not None:
-        _dense(bias, "bias", torch.float32, (N,))
-    if activation not in ACTIVATIONS:
+    sap, sbp = _dense(scale_a, "scale_a", device, torch.float32, (M,)), _dense(scale_b, "scale_b", device, torch.float32, (N,))
+    biasp = None if bias is None else _dense(bias, "bias", device, torch.float32, (N,))
+    act = ACTIVATIONS.get(activation)
+    if act is None:
         raise FvsrnError(-1, "unknown activation %r" % (activation,))
     if dtype is None:
         dtype = torch.float32 if out is None else out.dtype
-    if str(dtype) not in _TENSOR_DTYPES:
+    code = _tensor_dtypes().get(dtype)
+    if code is None:
         raise FvsrnError(-1, "the output must be float32, float16 or bfloat16")
-    with _OnStream(stream) as s:
-        if out is None:
-            out = torch.empty((M, N), dtype=dtype, device=a.device)
-        ldo = _rows(_operand(out, "out", dtype, (M, N)), "out")
-        _check(lib().fvsrn_matmul_int8(a.data_ptr(), lda, scale_a.data_ptr(), b.data_ptr(), ldb, scale_b.data_ptr(), None if bias is None else bias.data_ptr(), M, N, K,
-                                       ACTIVATIONS[activation], float(activation_param), out.data_ptr(), _TENSOR_DTYPES[str(dtype)], ldo, s))
+    if out is None:
+        out = _allocated(context, lambda: torch.empty((M, N), dtype=dtype, device=a.device))
+    op = _operand(out, "out", device, dtype, (M, N))
+    _check(lib().fvsrn_matmul_int8(ap, lda, sap, bp, ldb, sbp, biasp, M, N, K, act, activation_param, op, code, _row_stride(out, "out"), s))
     return out
 
 
-def _scan_desc(gate, x, gate_mode, gate_scale, input_mode, reverse, h0, lengths):
-    import torch
-    _operand(gate, "gate")
-    if str(gate.dtype) not in _TENSOR_DTYPES:
-        raise FvsrnError(-1, "gate must be float32, float16 or bfloat16")
-    _operand(x, "x", gate.dtype)
-    if gate.dim() != 3 or x.dim() != 3 or gate.shape[:2] != x.shape[:2]:
+@functools.lru_cache(maxsize=512)
+def _scan_plan(code, gate_mode, gate_scale, input_mode, reverse, gate_shape, x_shape, gate_stride, x_stride, out_stride, dout_stride, dgate_stride, dx_stride):
+    """The description of a scan of these shapes and strides (None: that operand is not there) and the bytes of scratch memory it needs."""
+    if len(gate_shape) != 3 or len(x_shape) != 3 or gate_shape[:2] != x_shape[:2]:
         raise FvsrnError(-1, "gate must be (batch, steps, gate channels) and x (batch, steps, channels)")
-    d = ScanDesc()
-    d.dtype, d.gate_mode, d.input_mode, d.reverse, d.gate_scale = _TENSOR_DTYPES[str(gate.dtype)], gate_mode, input_mode, int(reverse), gate_scale
-    d.batch, d.length, d.channels, d.gate_channels = x.shape[0], x.shape[1], x.shape[2], gate.shape[2]
-    d.gate_stride[:], d.x_stride[:] = gate.stride(), x.stride()
-    if h0 is not None:
-        _dense(h0, "h0", torch.float32, (x.shape[0], x.shape[2]))
-    if lengths is not None:
-        _dense(lengths, "lengths", torch.int32, (x.shape[0],))
-    return d
-
-
-def _scan_workspace(d, backward, device):
-    import torch
+    d = ScanDesc(dtype=code, gate_mode=gate_mode, input_mode=input_mode, reverse=int(reverse), gate_scale=gate_scale, length=x_shape[1], batch=x_shape[0],
+                 channels=x_shape[2], gate_channels=gate_shape[2])
+    for name, stride in (("gate_stride", gate_stride), ("x_stride", x_stride), ("out_stride", out_stride), ("dout_stride", dout_stride),
+                         ("dgate_stride", dgate_stride), ("dx_stride", dx_stride)):
+        if stride is not None:
+            getattr(d, name)[:] = stride
     n = _SZ(0)
-    _check(lib().fvsrn_gated_scan_workspace(C.byref(d), backward, C.byref(n)))
-    return (torch.empty(n.value, dtype=torch.uint8, device=device) if n.value else None), n.value
-
-
-def _ptr(t):
-    return None if t is None else t.data_ptr()
+    _check(lib().fvsrn_gated_scan_workspace(C.byref(d), int(dx_stride is not None), C.byref(n)))
+    return d, C.byref(d), n.value
 
 
 def gated_scan(gate, x, *, gate_mode: int = GATE_VALUE, gate_scale: float = 1.0, input_mode: int = INPUT_ADD, reverse: bool = False, h0=None, lengths=None,
@@ -864,17 +868,25 @@ def gated_scan(gate, x, *, gate_mode: int = GATE_VALUE, gate_scale: float = 1.0,
     Beer-Lambert blending of the colours (rays, samples, rgb + absorption) that Scene.evaluate_tf gives, back to front:
         _, rgb = gated_scan(c[..., 3:], c[..., :3], gate_mode=GATE_EXP, gate_scale=-stepsize, input_mode=INPUT_BLEND, reverse=True, states=False)"""
     import torch
-    d = _scan_desc(gate, x, gate_mode, gate_scale, input_mode, reverse, h0, lengths)
-    with _OnStream(stream) as s:
-        if out is None and states:
-            out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        if last is None:
-            last = torch.empty((x.shape[0], x.shape[2]), dtype=torch.float32, device=x.device)
-        _dense(last, "last", torch.float32, (x.shape[0], x.shape[2]))
-        if out is not None:
-            d.out_stride[:] = _operand(out, "out", x.dtype, x.shape).stride()
-        ws, n = _scan_workspace(d, 0, x.device)
-        _check(lib().fvsrn_gated_scan(C.byref(d), gate.data_ptr(), x.data_ptr(), _ptr(h0), _ptr(lengths), _ptr(out), last.data_ptr(), _ptr(ws), n, s))
+    device, s, context = _launch_state(gate, "gate", stream)
+    dtype = getattr(gate, "dtype", None)
+    code = _tensor_dtypes().get(dtype)
+    if code is None:
+        raise FvsrnError(-1, "gate must be float32, float16 or bfloat16")
+    gp, xp = _operand(gate, "gate", device, dtype), _operand(x, "x", device, dtype)
+    shape = x.shape
+    if out is None and states:
+        out = _allocated(context, lambda: torch.empty(shape, dtype=dtype, device=x.device))
+    op = None if out is None else _operand(out, "out", device, dtype, shape)
+    _, ref, bytes_ = _scan_plan(code, gate_mode, gate_scale, input_mode, reverse, gate.shape, shape, gate.stride(), x.stride(), None if out is None else out.stride(), None, None, None)
+    ends = (shape[0], shape[2])
+    if last is None:
+        last = _allocated(context, lambda: torch.empty(ends, dtype=torch.float32, device=x.device))
+    lp = _dense(last, "last", device, torch.float32, ends)
+    hp = None if h0 is None else _dense(h0, "h0", device, torch.float32, ends)
+    np_ = None if lengths is None else _dense(lengths, "lengths", device, torch.int32, ends[:1])
+    ws = _allocated(context, lambda: torch.empty(bytes_, dtype=torch.uint8, device=x.device)) if bytes_ else None
+    _check(lib().fvsrn_gated_scan(ref, gp, xp, hp, np_, op, lp, None if ws is None else ws.data_ptr(), bytes_, s))
     return out, last
 
 
@@ -883,23 +895,28 @@ def gated_scan_backward(gate, x, dout=None, dlast=None, *, gate_mode: int = GATE
     """Gradients (dgate, dx, dh0) of gated_scan with the same arguments for dout (of the states) and / or dlast (of the last state, float32); dh0 is None without
     h0 (fvsrn_gated_scan_backward).  Inputs that were broadcast (expand) get their gradient per element."""
     import torch
-    d = _scan_desc(gate, x, gate_mode, gate_scale, input_mode, reverse, h0, lengths)
-    if dout is not None:
-        d.dout_stride[:] = _operand(dout, "dout", x.dtype, x.shape).stride()
-    if dlast is not None:
-        _dense(dlast, "dlast", torch.float32, (x.shape[0], x.shape[2]))
-    with _OnStream(stream) as s:
-        if dgate is None:
-            dgate = torch.empty(gate.shape, dtype=gate.dtype, device=gate.device)
-        if dx is None:
-            dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        if dh0 is None and h0 is not None:
-            dh0 = torch.empty_like(h0)
-        if dh0 is not None:
-            _dense(dh0, "dh0", torch.float32, (x.shape[0], x.shape[2]))
-        d.dgate_stride[:] = _operand(dgate, "dgate", gate.dtype, gate.shape).stride()
-        d.dx_stride[:] = _operand(dx, "dx", x.dtype, x.shape).stride()
-        ws, n = _scan_workspace(d, 1, x.device)
-        _check(lib().fvsrn_gated_scan_backward(C.byref(d), gate.data_ptr(), x.data_ptr(), _ptr(h0), _ptr(lengths), _ptr(dout), _ptr(dlast), dgate.data_ptr(),
-                                               dx.data_ptr(), _ptr(dh0), _ptr(ws), n, s))
+    device, s, context = _launch_state(gate, "gate", stream)
+    dtype = getattr(gate, "dtype", None)
+    code = _tensor_dtypes().get(dtype)
+    if code is None:
+        raise FvsrnError(-1, "gate must be float32, float16 or bfloat16")
+    gp, xp = _operand(gate, "gate", device, dtype), _operand(x, "x", device, dtype)
+    shape = x.shape
+    if dgate is None:
+        dgate = _allocated(context, lambda: torch.empty(gate.shape, dtype=dtype, device=x.device))
+    if dx is None:
+        dx = _allocated(context, lambda: torch.empty(shape, dtype=dtype, device=x.device))
+    dp = None if dout is None else _operand(dout, "dout", device, dtype, shape)
+    dgp, dxp = _operand(dgate, "dgate", device, dtype, gate.shape), _operand(dx, "dx", device, dtype, shape)
+    _, ref, bytes_ = _scan_plan(code, gate_mode, gate_scale, input_mode, reverse, gate.shape, shape, gate.stride(), x.stride(), None, None if dout is None else dout.stride(),
+                                dgate.stride(), dx.stride())
+    ends = (shape[0], shape[2])
+    if dh0 is None and h0 is not None:
+        dh0 = _allocated(context, lambda: torch.empty(ends, dtype=torch.float32, device=x.device))
+    dlp = None if dlast is None else _dense(dlast, "dlast", device, torch.float32, ends)
+    hp = None if h0 is None else _dense(h0, "h0", device, torch.float32, ends)
+    np_ = None if lengths is None else _dense(lengths, "lengths", device, torch.int32, ends[:1])
+    dhp = None if dh0 is None else _dense(dh0, "dh0", device, torch.float32, ends)
+    ws = _allocated(context, lambda: torch.empty(bytes_, dtype=torch.uint8, device=x.device)) if bytes_ else None
+    _check(lib().fvsrn_gated_scan_backward(ref, gp, xp, hp, np_, dp, dlp, dgp, dxp, dhp, None if ws is None else ws.data_ptr(), bytes_, s))
     return dgate, dx, dh0

@@ -493,8 +493,8 @@ int fvsrn_render_volume(fvsrn_scene* scene, fvsrn_volume* volume, int source, in
  * except where an entry says so.  A size of zero is a call that does nothing more than its definition says (no rows: nothing). */
 typedef enum { FVSRN_TENSOR_F32 = 0, FVSRN_TENSOR_F16 = 1, FVSRN_TENSOR_BF16 = 2 } fvsrn_tensor_dtype;
 
-/* Codes and scales of the rows of a matrix x [rows][cols] (row stride ldx): scale = max(max_k |x_k| / 127, 2^-126), code = x / scale rounded
- * to the nearest integer, ties to even; quotients are rounded to 32 bits.  A row that holds an infinity or a NaN gets the scale NaN and codes 0, so
+/* Codes and scales of the rows of a matrix x [rows][cols] (row stride ldx): scale = max(max_k |x_k| * f, 2^-126) with the 32-bit float f
+ * next to 1 / 127, code = x / scale (rounded to 32 bits) rounded to the nearest integer, ties to even.  A row that holds an infinity or a NaN gets the scale NaN and codes 0, so
  * that every product with it is NaN.  For tokens (the rows of an activation matrix) and for the channels of a layer (the rows of its
  * [out][in] weights) alike.  d_codes [rows][cols] with row stride ldc, d_scales [rows]. */
 int fvsrn_quantize_rows(const void* d_x, int dtype, long long rows, int cols, long long ldx, signed char* d_codes, long long ldc,

@@ -363,7 +363,7 @@ def plain_codes(x):
     """The definition, in numpy float32 (its divisions are rounded to 32 bits there too)."""
     v = x.float().cpu().numpy()
     bad = ~np.isfinite(v).all(1)
-    scale = np.maximum(np.abs(np.where(np.isfinite(v), v, 0)).max(1) / np.float32(127), np.float32(2.0 ** -126))
+    scale = np.maximum(np.abs(np.where(np.isfinite(v), v, 0)).max(1) * (np.float32(1) / np.float32(127)), np.float32(2.0 ** -126))
     q = np.where(bad[:, None], 0, np.rint(np.where(bad[:, None], 0, v) / scale[:, None]))
     return q.astype(np.int8), np.where(bad, np.float32(np.nan), scale)
 
