@@ -113,15 +113,35 @@ __device__ __forceinline__ float sineOfTurns(double v) {
 }
 
 // The activations of the network kernels (renderer_activations.cuh) on 32-bit floats
-__device__ __forceinline__ float activated(float y, int kind, float p) {
+template <int KIND>
+__device__ __forceinline__ float activated(float y, float p) {
     constexpr double kTurn = 0.15915494309189535;  // 1 / (2 pi)
+    if constexpr (KIND == FVSRN_ACT_RELU) {
+        return y < 0.f ? 0.f : y;  // (NaN stays NaN)
+    } else if constexpr (KIND == FVSRN_ACT_SINE) {
+        return sineOfTurns(double(p * y) * kTurn);
+    } else if constexpr (KIND == FVSRN_ACT_SNAKE) {
+        const float s = sineOfTurns(double(p * y) * kTurn);
+        return y + s * s / p;
+    } else if constexpr (KIND == FVSRN_ACT_SNAKEALT) {
+        return (y + 1.f - sineOfTurns(double(2.f * p * y) * kTurn + 0.25)) / (2.f * p);
+    } else if constexpr (KIND == FVSRN_ACT_SIGMOID) {
+        return 1.f / (1.f + expf(-y));
+    } else {
+        return y;
+    }
+}
+
+// f(activation as a constant): one wave-uniform branch in front of the outputs of a wave
+template <class F>
+__device__ __forceinline__ void withActivation(int kind, F&& f) {
     switch (kind) {
-        case FVSRN_ACT_RELU: return y < 0.f ? 0.f : y;  // (NaN stays NaN)
-        case FVSRN_ACT_SINE: return sineOfTurns(double(p * y) * kTurn);
-        case FVSRN_ACT_SNAKE: { const float s = sineOfTurns(double(p * y) * kTurn); return y + s * s / p; }
-        case FVSRN_ACT_SNAKEALT: return (y + 1.f - sineOfTurns(double(2.f * p * y) * kTurn + 0.25)) / (2.f * p);
-        case FVSRN_ACT_SIGMOID: return 1.f / (1.f + expf(-y));
-        default: return y;
+        case FVSRN_ACT_RELU: return f(std::integral_constant<int, FVSRN_ACT_RELU>{});
+        case FVSRN_ACT_SINE: return f(std::integral_constant<int, FVSRN_ACT_SINE>{});
+        case FVSRN_ACT_SNAKE: return f(std::integral_constant<int, FVSRN_ACT_SNAKE>{});
+        case FVSRN_ACT_SNAKEALT: return f(std::integral_constant<int, FVSRN_ACT_SNAKEALT>{});
+        case FVSRN_ACT_SIGMOID: return f(std::integral_constant<int, FVSRN_ACT_SIGMOID>{});
+        default: return f(std::integral_constant<int, FVSRN_ACT_NONE>{});
     }
 }
 
@@ -145,8 +165,9 @@ __device__ __forceinline__ int4_t loadCodes(const signed char* row, int k, int K
     return v;
 }
 
-__device__ __forceinline__ float scaled(int acc, float sa, float sb, float bias, int activation, float param) {
-    return activated(fmaf(float(acc) * sb, sa, bias), activation, param);
+template <int KIND>
+__device__ __forceinline__ float scaled(int acc, float sa, float sb, float bias, float param) {
+    return activated<KIND>(fmaf(float(acc) * sb, sa, bias), param);
 }
 
 // Few tokens: bound by the weights' bytes, or by how long one wave takes through its part of k.  v_mfma_i32_16x16x64_i8 with the weights as its rows: lane l holds 16
@@ -189,11 +210,14 @@ __global__ __launch_bounds__(512) void matmul_int8_few_kernel(const Int8Params p
         const long long m = m0 + t * 16 + col;
         if (m >= p.M) continue;
         const float sa = p.scaleA[m];
+        withActivation(activation, [&](auto kind) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int n = n0 + part * 4 + r;
-            if (n < p.N) static_cast<T*>(p.out)[m * p.ldo + n] = fromFloat<T>(scaled(s[r], sa, p.scaleB[n], p.bias ? p.bias[n] : 0.f, activation, p.actParam));
-        }
+            for (int r = 0; r < 4; ++r) {
+                const int n = n0 + part * 4 + r;
+                if (n < p.N)
+                    static_cast<T*>(p.out)[m * p.ldo + n] = fromFloat<T>(scaled<decltype(kind)::value>(s[r], sa, p.scaleB[n], p.bias ? p.bias[n] : 0.f, p.actParam));
+            }
+        });
     }
 }
 
@@ -227,24 +251,33 @@ __global__ __launch_bounds__(256) void matmul_int8_kernel(const Int8Params p, co
     const int n = n0 + wn + col;
     if (n >= p.N) return;
     const float sb = p.scaleB[n], bias = p.bias ? p.bias[n] : 0.f;
+    float sa[16];
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-        const long long m = m0 + wm + 8 * (r >> 2) + 4 * half + (r & 3);
-        if (m < p.M) static_cast<T*>(p.out)[m * p.ldo + n] = fromFloat<T>(scaled(acc[r], p.scaleA[m], sb, bias, activation, p.actParam));
-    }
+    for (int r = 0; r < 16; ++r) sa[r] = p.scaleA[min(m0 + wm + 8 * (r >> 2) + 4 * half + (r & 3), p.M - 1)];
+    withActivation(activation, [&](auto kind) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const long long m = m0 + wm + 8 * (r >> 2) + 4 * half + (r & 3);
+            if (m < p.M) static_cast<T*>(p.out)[m * p.ldo + n] = fromFloat<T>(scaled<decltype(kind)::value>(acc[r], sa[r], sb, bias, p.actParam));
+        }
+    });
 }
 
-// Aligned rows: a tile of TM tokens x TN channels for WM x WN waves of 32 x 32 pieces, 128 bytes of k at a time, which go from memory into LDS without passing
-// a register (two buffers: the next 128 bytes travel while these are multiplied).  LDS holds rows of eight 16-byte chunks, chunk c of row r at place c ^ swizzle(r) so that
-// the 32 rows a wave reads at one k spread over all banks; the loads write LDS in lane order, so it is their source that is permuted.
-// A wave's channels are paired -- column l of its piece j is channel 2 l + j -- so that a lane stores two adjacent outputs.
+// Aligned rows: a tile of TM tokens x TN channels for WM x WN waves, each with PM x 2 pieces of 32 x 32, 64 bytes of k a stage.
+//   Stages go from memory into LDS without passing a register, into a ring of four: while one is multiplied three travel (a stage of 256 x 256 is multiplied in
+// 0.4 us, which is less than the way from memory).  The wait for the next stage and the barrier stand between the two halves of a stage's products, and the
+// operands of a half are read while the half before is multiplied, so the matrix units have work queued at every wait.
+//   LDS holds rows of four 16-byte chunks, chunk c of row r at place c ^ swizzle(r), so that the 32 rows a wave reads at one k spread over all banks; the
+// loads write LDS in lane order, so it is their source that is permuted.  A wave's channels are paired -- column l of its piece j is channel 2 l + j -- so that a
+// lane stores two adjacent outputs and a wave whole 128-byte lines of 16-bit ones.
 template <class T, int TM, int TN, int WM, int WN>
 __global__ __launch_bounds__(64 * WM * WN) void matmul_int8_tile_kernel(const Int8Params p, const int activation, const int tilesM, const int tilesN) {
-    constexpr int BK = 128, WAVES = WM * WN, PM = TM / WM / 32, PN = TN / WN / 32;
-    static_assert(PN == 2, "a wave's channels are paired");
-    constexpr int LOADS = (TM + TN) * BK / (64 * 16) / WAVES;  // 1 KiB each: eight rows
-    static_assert((TM + TN) / 8 % WAVES == 0 && TM / 8 % LOADS == 0, "a wave's loads are all tokens' or all channels'");
-    __shared__ __attribute__((aligned(1024))) signed char lds[2][(TM + TN) * BK];
+    constexpr int BK = 64, RING = 4, WAVES = WM * WN, PM = TM / WM / 32, STAGE = (TM + TN) * BK;
+    static_assert(TN / WN == 64, "a wave's channels are paired");
+    constexpr int LOADS = STAGE / 1024 / WAVES;  // of a wave, 1 KiB each: 16 rows
+    static_assert(LOADS == 4, "the waits below count loads");
+    __shared__ __attribute__((aligned(1024))) signed char lds[RING][STAGE];
+    __shared__ __attribute__((aligned(16))) float scaleA[TM], scaleB[TN], bias[TN];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // Tiles of an XCD (workgroup id % 8) are neighbours, in columns of up to eight tiles of tokens: what one reads the others find in its L2.
     const unsigned tiles = unsigned(tilesM) * tilesN, id = blockIdx.x, share = tiles / 8, more = tiles % 8, xcd = id % 8;
@@ -253,90 +286,118 @@ __global__ __launch_bounds__(64 * WM * WN) void matmul_int8_tile_kernel(const In
     const long long m0 = (long long)(band * 8 + inBand % bandRows) * TM;
     const int n0 = int(inBand / bandRows) * TN;
 
-    const int lr = lane >> 3;
     const signed char* source[LOADS];
     int chunk[LOADS];
 #pragma unroll
     for (int j = 0; j < LOADS; ++j) {
-        const int row = (wave * LOADS + j) * 8 + lr;  // of the tile: tokens, then channels
-        if (row < TM) {
-            chunk[j] = ((lane & 7) ^ (row & 7)) * 16;
-            source[j] = p.a + min(m0 + row, p.M - 1) * p.lda;
-        } else {
-            chunk[j] = ((lane & 7) ^ ((row >> 1) & 7)) * 16;
-            source[j] = p.b + (long long)min(n0 + row - TM, p.N - 1) * p.ldb;
-        }
+        const int row = (wave * LOADS + j) * 16 + (lane >> 2);  // of the tile: tokens, then channels
+        const bool token = row < TM;
+        chunk[j] = ((lane & 3) ^ ((token ? row >> 1 : row >> 2) & 3)) * 16;
+        source[j] = (token ? p.a + min(m0 + row, p.M - 1) * p.lda : p.b + (long long)min(n0 + row - TM, p.N - 1) * p.ldb) + chunk[j];
     }
-    auto load = [&](int k0, int buffer) {
+    const int stages = (p.K + BK - 1) / BK;
+    auto load = [&](int stage) {
 #pragma unroll
         for (int j = 0; j < LOADS; ++j) {
-            const int k = k0 + chunk[j];
-            // (a chunk behind the row's end is never multiplied: any address will do)
-            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(source[j] + (k < p.K ? k : 0)),
-                                             (__attribute__((address_space(3))) void*)(&lds[buffer][(wave * LOADS + j) * 1024]), 16, 0, 0);
+            const int k = stage * BK;
+            // (a chunk behind the row's end meets zeros in the other operand: any address of the row will do)
+            const signed char* const from = source[j] + (k + chunk[j] < p.K ? k : -chunk[j]);
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
+                                             (__attribute__((address_space(3))) void*)(&lds[stage % RING][(wave * LOADS + j) * 1024]), 16, 0, 0);
         }
     };
-    const int wm = (wave / WN) * (PM * 32), wn = (wave % WN) * (PN * 32), col = lane & 31, half = lane >> 5;
-    int16_t_ acc[PM][PN] = {};
-    auto multiply = [&](int buffer, int kk, bool cut) {
-        int4_t a[PM], b[PN];
+    const int wm = (wave / WN) * (PM * 32), wn = (wave % WN) * 64, col = lane & 31, half = lane >> 5;
+    struct Operands { int4_t a[PM], b[2]; };
+    auto read = [&](Operands& o, int stage, int kk) {
+        const signed char* const buffer = lds[stage % RING];
 #pragma unroll
         for (int i = 0; i < PM; ++i) {
             const int row = wm + i * 32 + col;
-            a[i] = *reinterpret_cast<const int4_t*>(&lds[buffer][row * BK + (((kk * 2 + half) ^ (row & 7)) * 16)]);
+            o.a[i] = *reinterpret_cast<const int4_t*>(buffer + row * BK + (((kk * 2 + half) ^ ((row >> 1) & 3)) * 16));
         }
 #pragma unroll
-        for (int j = 0; j < PN; ++j) {
-            const int row = wn + 2 * col + j;
-            b[j] = *reinterpret_cast<const int4_t*>(&lds[buffer][(TM + row) * BK + (((kk * 2 + half) ^ ((row >> 1) & 7)) * 16)]);
-            if (cut && half) b[j] = int4_t{0, 0, 0, 0};  // K ends in the middle of this step
+        for (int j = 0; j < 2; ++j) {
+            const int row = TM + wn + 2 * col + j;
+            o.b[j] = *reinterpret_cast<const int4_t*>(buffer + row * BK + (((kk * 2 + half) ^ ((row >> 2) & 3)) * 16));
         }
+    };
+    int16_t_ acc[PM][2] = {};
+    auto multiply = [&](const Operands& o) {
 #pragma unroll
         for (int i = 0; i < PM; ++i)
 #pragma unroll
-            for (int j = 0; j < PN; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(a[i], b[j], acc[i][j], 0, 0, 0);
+            for (int j = 0; j < 2; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(o.a[i], o.b[j], acc[i][j], 0, 0, 0);
     };
-    load(0, 0);
-    int buffer = 0, k0 = 0;
-    for (; k0 + BK <= p.K; k0 += BK, buffer ^= 1) {
-        __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wave's part of the tile is in LDS
-        __syncthreads();                     // everybody's is, and nobody reads the other buffer any more
-        if (k0 + BK < p.K) load(k0 + BK, buffer ^ 1);
-#pragma unroll
-        for (int kk = 0; kk < BK / 32; ++kk) multiply(buffer, kk, false);
+    for (int e = threadIdx.x; e < TM; e += 64 * WAVES) scaleA[e] = p.scaleA[min(m0 + e, p.M - 1)];
+    for (int e = threadIdx.x; e < TN; e += 64 * WAVES) {
+        const int n = min(n0 + e, p.N - 1);
+        scaleB[e] = p.scaleB[n];
+        bias[e] = p.bias ? p.bias[n] : 0.f;
     }
-    if (k0 < p.K) {
-        __builtin_amdgcn_s_waitcnt(0x0f70);
-        __syncthreads();
+    // The next stage is everybody's to read behind the barrier, and nobody reads the one before it any more.  Two stages may still be on their way (8
+    // loads of this wave); at the end of k all have to be there.
+    auto arrive = [&](bool flowing) {
+        if (flowing) __builtin_amdgcn_s_waitcnt(0x0078);  // vmcnt(8) lgkmcnt(0)
+        else __builtin_amdgcn_s_waitcnt(0x0070);          // vmcnt(0) lgkmcnt(0)
+        asm volatile("s_barrier" ::: "memory");
+    };
+    for (int s = 0; s < min(RING - 1, stages); ++s) load(s);
+    arrive(stages >= RING - 1);
+    Operands even, odd;
+    read(even, 0, 0);
 #pragma unroll 1
-        for (int left = p.K - k0, kk = 0; kk * 32 < left; ++kk) multiply(buffer, kk, left - kk * 32 < 32);
+    for (int s = 0; s < stages - 1; ++s) {
+        if (s + RING - 1 < stages) load(s + RING - 1);
+        read(odd, s, 1);
+        multiply(even);
+        arrive(s + RING - 1 < stages);
+        read(even, s + 1, 0);
+        multiply(odd);
     }
-    const int n = n0 + wn + 2 * col;
-    float sb[2], bias[2];
+    // the last stage: zeros in the place of what lies behind K
+    read(odd, stages - 1, 1);
+    const int left = p.K - (stages - 1) * BK;
+    const int4_t zero = {0, 0, 0, 0};
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-        const int c = min(n + j, p.N - 1);
-        sb[j] = p.scaleB[c];
-        bias[j] = p.bias ? p.bias[c] : 0.f;
+        even.b[j] = half * 16 < left ? even.b[j] : zero;
+        odd.b[j] = 32 + half * 16 < left ? odd.b[j] : zero;
     }
-    const bool paired = n + 1 < p.N && p.ldo % 2 == 0 && reinterpret_cast<size_t>(p.out) % (2 * sizeof(T)) == 0;
+    multiply(even);
+    multiply(odd);
+    const int cn = wn + 2 * col, n = n0 + cn;
+    const float sb0 = scaleB[cn], sb1 = scaleB[cn + 1], bias0 = bias[cn], bias1 = bias[cn + 1];
+    const bool paired = p.ldo % 2 == 0 && reinterpret_cast<size_t>(p.out) % (2 * sizeof(T)) == 0;
+    T* const out = static_cast<T*>(p.out) + (m0 + wm + 4 * half) * p.ldo + n;
+    const long long rows = p.M - (m0 + wm + 4 * half);
+    auto store = [&](auto kind, auto isWhole) {
 #pragma unroll
-    for (int i = 0; i < PM; ++i)
+        for (int i = 0; i < PM; ++i)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            const long long m = m0 + wm + i * 32 + 8 * (r >> 2) + 4 * half + (r & 3);
-            if (m >= p.M) continue;
-            const float sa = p.scaleA[m];
-            T* const out = static_cast<T*>(p.out) + m * p.ldo + n;
-            Pack<T, 2> o;
+            for (int q = 0; q < 4; ++q) {
+                const float4 sa = *reinterpret_cast<const float4*>(&scaleA[wm + i * 32 + 8 * q + 4 * half]);
 #pragma unroll
-            for (int j = 0; j < 2; ++j) o.v[j] = fromFloat<T>(scaled(acc[i][j][r], sa, sb[j], bias[j], activation, p.actParam));
-            if (paired) *reinterpret_cast<Pack<T, 2>*>(out) = o;
-            else {
-                if (n < p.N) out[0] = o.v[0];
-                if (n + 1 < p.N) out[1] = o.v[1];
+                for (int r = 0; r < 4; ++r) {
+                    constexpr int A = decltype(kind)::value;
+                    const int row = i * 32 + 8 * q + r;
+                    const float s = r == 0 ? sa.x : r == 1 ? sa.y : r == 2 ? sa.z : sa.w;
+                    Pack<T, 2> o;
+                    o.v[0] = fromFloat<T>(scaled<A>(acc[i][0][4 * q + r], s, sb0, bias0, p.actParam));
+                    o.v[1] = fromFloat<T>(scaled<A>(acc[i][1][4 * q + r], s, sb1, bias1, p.actParam));
+                    T* const to = out + row * p.ldo;
+                    if (decltype(isWhole)::value) {
+                        *reinterpret_cast<Pack<T, 2>*>(to) = o;
+                    } else if (row < rows) {
+                        if (n < p.N) to[0] = o.v[0];
+                        if (n + 1 < p.N) to[1] = o.v[1];
+                    }
+                }
             }
-        }
+    };
+    withActivation(activation, [&](auto kind) {
+        if (paired && m0 + TM <= p.M && n0 + TN <= p.N) store(kind, std::true_type{});
+        else store(kind, std::false_type{});
+    });
 }
 
 int powerOfTwoAtLeast(long long v) {
@@ -389,18 +450,16 @@ hipError_t launch_matmul_int8(const Int8Params& p, int activation, int outDtype,
             if (p.M <= 32) return few(isAligned, std::integral_constant<int, 2>{});
             return few(isAligned, std::integral_constant<int, 4>{});
         };
-        if (p.M <= 256) return aligned ? fewOf(std::true_type{}) : fewOf(std::false_type{});
-        const long long big = ((p.M + 255) / 256) * ((p.N + 255) / 256);
-        if (aligned && p.N > 64) {
-            if (big >= 256 && p.K >= 1024) {
-                matmul_int8_tile_kernel<T, 256, 256, 2, 4><<<unsigned(big), 512, 0, s>>>(p, activation, int((p.M + 255) / 256), (p.N + 255) / 256);
-                return hipGetLastError();
-            }
-            const long long tilesM = (p.M + 127) / 128, tilesN = (p.N + 127) / 128;
-            if (tilesM * tilesN < (1LL << 24)) {
-                matmul_int8_tile_kernel<T, 128, 128, 2, 2><<<unsigned(tilesM * tilesN), 256, 0, s>>>(p, activation, int(tilesM), int(tilesN));
-                return hipGetLastError();
-            }
+        if (p.M <= 64) return aligned ? fewOf(std::true_type{}) : fewOf(std::false_type{});
+        auto tiles = [&](int edge) { return ((p.M + edge - 1) / edge) * ((p.N + edge - 1) / edge); };
+        if (aligned && p.N > 32 && tiles(64) < (1LL << 24)) {
+            if (tiles(256) >= 256 && p.K >= 1024)
+                matmul_int8_tile_kernel<T, 256, 256, 2, 4><<<unsigned(tiles(256)), 512, 0, s>>>(p, activation, int((p.M + 255) / 256), (p.N + 255) / 256);
+            else if (tiles(128) >= 256)
+                matmul_int8_tile_kernel<T, 128, 128, 2, 2><<<unsigned(tiles(128)), 256, 0, s>>>(p, activation, int((p.M + 127) / 128), (p.N + 127) / 128);
+            else
+                matmul_int8_tile_kernel<T, 64, 64, 2, 1><<<unsigned(tiles(64)), 128, 0, s>>>(p, activation, int((p.M + 63) / 64), (p.N + 63) / 64);
+            return hipGetLastError();
         }
         const dim3 grid(unsigned((p.M + 63) / 64), unsigned((p.N + 63) / 64));
         if (aligned) matmul_int8_kernel<T, true><<<grid, 256, 0, s>>>(p, activation);
