@@ -852,8 +852,7 @@ def _scan_plan(code, gate_mode, gate_scale, input_mode, reverse, gate_shape, x_s
                  channels=x_shape[2], gate_channels=gate_shape[2])
     for name, stride in (("gate_stride", gate_stride), ("x_stride", x_stride), ("out_stride", out_stride), ("dout_stride", dout_stride),
                          ("dgate_stride", dgate_stride), ("dx_stride", dx_stride)):
-        if stride is not None:
-            getattr(d, name)[:] = stride
+        getattr(d, name)[:] = (0, 0, 1) if stride is None else stride
     n = _SZ(0)
     _check(lib().fvsrn_gated_scan_workspace(C.byref(d), int(dx_stride is not None), C.byref(n)))
     return d, C.byref(d), n.value

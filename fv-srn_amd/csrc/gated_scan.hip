@@ -51,29 +51,31 @@ __device__ __forceinline__ int lengthOf(const ScanParams& p, long long b) {
 // step i of a sequence of n steps is at position t; behind the sequence (outputs are zero there) i is the position itself
 __device__ __forceinline__ int positionOf(int i, int n, int reverse) { return reverse && i < n ? n - 1 - i : i; }
 
-constexpr int kScanWaves = 8;    // channels: waves that share a tile
-constexpr int kForwardSteps = 16; // channels: steps of a wave held in registers
-constexpr int kBackwardSteps = 8;
-
 // ---------------------------------------------------------------------------------------------------------------------
 // lanes are channels
 // ---------------------------------------------------------------------------------------------------------------------
 
-// What a wave's lanes stand for.  slots == 1: 64 V adjacent channels.  Otherwise (backward) `slots` lanes of a gate's channels -- padded to a power of two, so
-// that their sum is a butterfly of shuffles -- and, for gates of more than 64 channels, `parts` waves.
+constexpr int kScanWaves = 8;  // waves that share a tile
+// steps of a wave that are held in registers, for V channels of a lane
+constexpr int forwardSteps(int V) { return V <= 2 ? 16 : 8; }
+constexpr int backwardSteps(int V) { return V <= 2 ? 8 : 4; }
+
+// What a lane stands for: V adjacent channels, each with a gate of its own, or (SHARED) the V channels of one gate.  V == 1 and slots > 1 (backward, gates
+// of many channels): `slots` lanes of a gate's channels -- padded to a power of two, so that their sum is a butterfly of shuffles -- and, for
+// gates of more than 64 channels, `parts` waves.
 struct ChannelLane {
     int c, g, part;
     bool live;
 };
-template <int V>
+template <int V, bool SHARED>
 __device__ __forceinline__ ChannelLane channelLane(const ScanParams& p, int block, int lane, int slots, int parts) {
     ChannelLane r;
     r.part = 0;
-    if (slots == 1) {
-        const long long c = (long long)(block * 64LL + lane) * V;
-        r.live = c < p.C;
-        r.c = int(min(c, (long long)(p.C - V)));
-        r.g = r.c / p.G;
+    if (V > 1 || slots == 1) {
+        const long long own = block * 64LL + lane, last = p.C / V - 1;
+        r.live = own <= last;
+        r.c = int(min(own, last)) * V;
+        r.g = SHARED ? r.c / V : V > 1 ? r.c : r.c / p.G;
     } else if (parts == 1) {
         const int j = lane & (slots - 1);
         const long long g = (long long)block * (64 / slots) + lane / slots;
@@ -89,35 +91,78 @@ __device__ __forceinline__ ChannelLane channelLane(const ScanParams& p, int bloc
     }
     return r;
 }
-inline long long channelBlocks(const ScanParams& p, int vec, int slots, int parts) {
-    if (slots == 1) return (p.C + 64LL * vec - 1) / (64LL * vec);
-    if (parts == 1) return (p.Cg + 64 / slots - 1) / (64 / slots);
-    return (long long)p.Cg * parts;
+inline long long channelBlocks(const ScanParams& p, const ScanPlan& plan) {
+    if (plan.slots == 1) return (p.C / plan.vec + 63LL) / 64;
+    if (plan.parts == 1) return (p.Cg + 64 / plan.slots - 1) / (64 / plan.slots);
+    return (long long)p.Cg * plan.parts;
 }
 
-// Forward.  AGGREGATE: only (A, U) of this workgroup's span, span 0 with h0 folded in (its A slot then holds h0 for the second launch: d_last may be d_h0).
-template <class T, bool EXP, bool BLEND, int NW, int V, bool AGGREGATE>
+// V channels of steps i .. i + L - 1, zeros from step `end` on
+template <class T, int V, int L>
+__device__ __forceinline__ void loadChannels(const T* p, long long step, int i, int n, int end, int reverse, T (&to)[L][V]) {
+    if (i + L <= end) {  // (the same for all lanes)
+        const T* at = p + positionOf(i, n, reverse) * step;
+        const long long next = reverse ? -step : step;
+#pragma unroll
+        for (int k = 0; k < L; ++k) loadWide<T, V>(to[k], at + k * next);
+    } else {
+#pragma unroll
+        for (int k = 0; k < L; ++k) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) to[k][v] = T(0.f);
+            if (i + k < end) loadWide<T, V>(to[k], p + positionOf(i + k, n, reverse) * step);
+        }
+    }
+}
+
+// The gates of steps i .. i + L - 1 (1 from step `end` on); rest: the factor of x, 1 - a of BLEND and 1 of ADD
+template <class T, int V, int L>
+__device__ __forceinline__ void gatesOf(const ScanParams& p, const T (&raw)[L][V], int i, int end, float (&a)[L][V], float (&rest)[L][V]) {
+    if (p.exp) {
+#pragma unroll
+        for (int k = 0; k < L; ++k)
+#pragma unroll
+            for (int v = 0; v < V; ++v) gateOf<true>(toFloat(raw[k][v]), p.scale, a[k][v], rest[k][v]);
+    } else {
+#pragma unroll
+        for (int k = 0; k < L; ++k)
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                gateOf<false>(toFloat(raw[k][v]), p.scale, a[k][v], rest[k][v]);
+                if (i + L > end && i + k >= end) a[k][v] = 1.f;  // (read as 0; a gate of 0 in EXP is 1 already, and x is 0)
+            }
+    }
+    if (!p.blend) {
+#pragma unroll
+        for (int k = 0; k < L; ++k)
+#pragma unroll
+            for (int v = 0; v < V; ++v) rest[k][v] = 1.f;
+    }
+}
+
+// Forward.  AGGREGATE: only (A, U) of this workgroup's span, span 0 with h0 folded in (its A slot then holds h0 for the second launch: d_last may be d_h0).  The second
+// launch takes the spans from the last to the first: what the first launch read last is what the memory-side cache still holds.
+template <class T, int NW, int V, bool SHARED, bool AGGREGATE>
 __global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW) void scan_channels_kernel(const ScanParams p, const ScanPlan plan, const int blocks, const long long units) {
-    constexpr int L = kForwardSteps;
+    constexpr int L = forwardSteps(V), GV = SHARED ? 1 : V;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int w = NW == 1 ? 0 : wave;
     const long long unit = NW == 1 ? blockIdx.x * 4LL + wave : blockIdx.x;
     if (unit >= units) return;  // (NW == 1 only, and nothing is joined across its waves)
     const long long b = unit / blocks;
-    const ChannelLane ch = channelLane<V>(p, int(unit % blocks), lane, 1, 1);
-    const int n = lengthOf(p, b), span = blockIdx.y;
-    const int begin = span * plan.chunkSteps, end = min(p.out ? p.T : n, begin + plan.chunkSteps);
+    const ChannelLane ch = channelLane<V, SHARED>(p, int(unit % blocks), lane, 1, 1);
+    const int n = lengthOf(p, b), span = AGGREGATE ? blockIdx.y : gridDim.y - 1 - blockIdx.y;
+    const int begin = span * plan.chunkSteps, end = min(p.out ? p.T : n, begin + plan.chunkSteps), inside = min(n, end);
     const T* const gp = static_cast<const T*>(p.gate) + b * p.gs[0] + ch.g * p.gs[2];
     const T* const xp = static_cast<const T*>(p.x) + b * p.xs[0] + ch.c * p.xs[2];
     T* const op = p.out ? static_cast<T*>(p.out) + b * p.os[0] + ch.c * p.os[2] : nullptr;
     const long long state = b * p.C + ch.c, stored = (b * plan.chunks) * p.C + ch.c, plane = p.B * plan.chunks * p.C;
-    float h[V], A[V];
+    float h[V], A[GV];
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-        A[v] = 1.f;
-        h[v] = 0.f;
-    }
-    if (span == 0 || plan.chunks == 1) {
+    for (int v = 0; v < V; ++v) h[v] = 0.f;
+#pragma unroll
+    for (int v = 0; v < GV; ++v) A[v] = 1.f;
+    if (span == 0 && (AGGREGATE || plan.chunks == 1)) {
         if (p.h0)
 #pragma unroll
             for (int v = 0; v < V; ++v) h[v] = p.h0[state + v];
@@ -136,84 +181,76 @@ __global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW) void scan_channels_kernel(
         } else {
 #pragma unroll
             for (int v = 0; v < V; ++v) h[v] = wu[v];
+#pragma unroll 4
             for (int s = 1; s < span; ++s)
 #pragma unroll
                 for (int v = 0; v < V; ++v) h[v] = fmaf(wa[(long long)s * p.C + v], h[v], wu[(long long)s * p.C + v]);
         }
     }
-    __shared__ float2 joined[NW == 1 ? 1 : 2][NW][NW == 1 ? 1 : 64 * V];
+    __shared__ float joined[NW == 1 ? 1 : 2][NW][GV + V][NW == 1 ? 1 : 64];
     int buffer = 0;
     for (int tile = begin; tile < end; tile += NW * L) {
         const int i0 = tile + w * L;
-        float m[L][V], u[L][V];
+        T rawG[L][GV], rawX[L][V];
+        loadChannels<T, GV, L>(gp, p.gs[1], i0, n, inside, p.reverse, rawG);
+        loadChannels<T, V, L>(xp, p.xs[1], i0, n, inside, p.reverse, rawX);
+        float a[L][GV], rest[L][GV], u[L][V], a2[GV], u2[V];
+        gatesOf<T, GV, L>(p, rawG, i0, inside, a, rest);
+#pragma unroll
+        for (int v = 0; v < V; ++v) u2[v] = 0.f;
+#pragma unroll
+        for (int v = 0; v < GV; ++v) a2[v] = 1.f;
 #pragma unroll
         for (int k = 0; k < L; ++k) {
-            const int i = i0 + k;
-            if (i < n && i < end) {
-                const long long t = positionOf(i, n, p.reverse);
-                const Pack<T, V> x = *reinterpret_cast<const Pack<T, V>*>(xp + t * p.xs[1]);
-                const Pack<T, V> g = *reinterpret_cast<const Pack<T, V>*>(gp + t * p.gs[1]);
-#pragma unroll
-                for (int v = 0; v < V; ++v) {
-                    m[k][v] = toFloat(g.v[v]);
-                    u[k][v] = toFloat(x.v[v]);
-                }
-            } else {
-#pragma unroll
-                for (int v = 0; v < V; ++v) m[k][v] = EXP ? 0.f : 1.f, u[k][v] = 0.f;
-            }
-        }
-        float a2[V], u2[V];
-#pragma unroll
-        for (int v = 0; v < V; ++v) a2[v] = 1.f, u2[v] = 0.f;
-#pragma unroll
-        for (int k = 0; k < L; ++k)
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                float rest;
-                gateOf<EXP>(m[k][v], p.scale, m[k][v], rest);
-                if (BLEND) u[k][v] *= rest;
-                if (NW > 1 || AGGREGATE) {
-                    u2[v] = fmaf(m[k][v], u2[v], u[k][v]);
-                    a2[v] *= m[k][v];
-                }
+                u[k][v] = rest[k][SHARED ? 0 : v] * toFloat(rawX[k][v]);
+                if (NW > 1 || AGGREGATE) u2[v] = fmaf(a[k][SHARED ? 0 : v], u2[v], u[k][v]);
             }
+            if (NW > 1 || AGGREGATE)
+#pragma unroll
+                for (int v = 0; v < GV; ++v) a2[v] *= a[k][v];
+        }
         float pre[V];
 #pragma unroll
         for (int v = 0; v < V; ++v) pre[v] = h[v];
         if constexpr (NW > 1) {
 #pragma unroll
-            for (int v = 0; v < V; ++v) joined[buffer][w][lane * V + v] = make_float2(a2[v], u2[v]);
+            for (int v = 0; v < GV; ++v) joined[buffer][w][v][lane] = a2[v];
+#pragma unroll
+            for (int v = 0; v < V; ++v) joined[buffer][w][GV + v][lane] = u2[v];
             __syncthreads();  // (one barrier a tile: the two buffers take turns, and a wave can only be one tile ahead)
 #pragma unroll
-            for (int j = 0; j < NW; ++j)
+            for (int j = 0; j < NW; ++j) {
+                float aj[GV];
+#pragma unroll
+                for (int v = 0; v < GV; ++v) {
+                    aj[v] = joined[buffer][j][v][lane];
+                    if (AGGREGATE) A[v] *= aj[v];
+                }
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
                     if (j == w) pre[v] = h[v];
-                    const float2 s = joined[buffer][j][lane * V + v];
-                    h[v] = fmaf(s.x, h[v], s.y);
-                    if (AGGREGATE) A[v] *= s.x;
+                    h[v] = fmaf(aj[SHARED ? 0 : v], h[v], joined[buffer][j][GV + v][lane]);
                 }
-            buffer ^= 1;
-        } else if constexpr (AGGREGATE) {
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                h[v] = fmaf(a2[v], h[v], u2[v]);
-                A[v] *= a2[v];
             }
+            buffer ^= 1;
         }
         if constexpr (!AGGREGATE) {
+            const bool whole = i0 + L <= inside;
+            const long long next = p.reverse ? -p.os[1] : p.os[1];
+            T* const at = op && whole ? op + positionOf(i0, n, p.reverse) * p.os[1] : op;
 #pragma unroll
             for (int k = 0; k < L; ++k) {
-                const int i = i0 + k;
+                T o[V];
 #pragma unroll
-                for (int v = 0; v < V; ++v) pre[v] = fmaf(m[k][v], pre[v], u[k][v]);
-                if (op && i < end && ch.live) {
-                    Pack<T, V> o;
-#pragma unroll
-                    for (int v = 0; v < V; ++v) o.v[v] = fromFloat<T>(i < n ? pre[v] : 0.f);
-                    *reinterpret_cast<Pack<T, V>*>(op + (long long)positionOf(i, n, p.reverse) * p.os[1]) = o;
+                for (int v = 0; v < V; ++v) {
+                    pre[v] = fmaf(a[k][SHARED ? 0 : v], pre[v], u[k][v]);
+                    o[v] = fromFloat<T>(whole || i0 + k < n ? pre[v] : 0.f);
                 }
+                if (!op || !ch.live) continue;
+                if (whole) storeWide<T, V>(at + k * next, o);
+                else if (i0 + k < end) storeWide<T, V>(op + positionOf(i0 + k, n, p.reverse) * p.os[1], o);
             }
             if constexpr (NW == 1) {
 #pragma unroll
@@ -226,7 +263,7 @@ __global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW) void scan_channels_kernel(
         float* const wa = p.ws + stored + (long long)span * p.C;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            if (span > 0) wa[v] = A[v];
+            if (span > 0) wa[v] = A[SHARED ? 0 : v];
             wa[plane + v] = h[v];
         }
     } else if (p.last && span == plan.chunks - 1) {
@@ -235,199 +272,328 @@ __global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW) void scan_channels_kernel(
     }
 }
 
-// Backward, first launch of a call that is cut into spans: A, U (span 0 from h0) and D of every span.
-template <class T, bool EXP, bool BLEND, int NW>
-__global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW) void scan_channels_spans_kernel(const ScanParams p, const ScanPlan plan, const int blocks, const long long units) {
-    constexpr int L = kBackwardSteps;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int w = NW == 1 ? 0 : wave;
-    const long long unit = NW == 1 ? blockIdx.x * 4LL + wave : blockIdx.x;
-    if (unit >= units) return;
-    const long long b = unit / blocks;
-    const ChannelLane ch = channelLane<1>(p, int(unit % blocks), lane, plan.slots, plan.parts);
+// Backward, scratch memory: for each span A, U (span 0 from h0) and D; then for each tile what its span's first steps up to it make of the state that enters the
+// span, h -> A h + U (a call of one span: A is not there, U the state itself); then the parts of gate sums.
+struct BackwardScratch {
+    float *spans, *heads, *partial;
+    long long plane, headPlane;
+};
+__host__ __device__ inline BackwardScratch backwardScratch(const ScanParams& p, const ScanPlan& plan) {
+    BackwardScratch r;
+    const int tilesOfSpan = plan.chunkSteps / plan.tile;
+    r.plane = plan.chunks > 1 ? p.B * plan.chunks * (long long)p.C : 0;
+    r.headPlane = tilesOfSpan > 1 ? p.B * plan.chunks * tilesOfSpan * (long long)p.C : 0;
+    r.spans = p.ws;
+    r.heads = p.ws + 3 * r.plane;
+    r.partial = r.heads + (plan.chunks > 1 ? 2 : 1) * r.headPlane;
+    return r;
+}
+inline size_t backwardFloats(const ScanParams& p, const ScanPlan& plan) {
+    ScanParams q = p;
+    q.ws = nullptr;
+    const size_t partial = plan.parts > 1 ? size_t(p.B) * p.T * p.Cg * plan.parts : 0;
+    const BackwardScratch s = backwardScratch(q, plan);
+    return size_t(3 * s.plane + (plan.chunks > 1 ? 2 : 1) * s.headPlane) + partial;
+}
+
+// Backward, first launch of a call that is cut into spans
+template <class T, int NW, int V, bool SHARED>
+__global__ __launch_bounds__(64 * NW) void scan_channels_spans_kernel(const ScanParams p, const ScanPlan plan, const int blocks) {
+    constexpr int L = backwardSteps(V), GV = SHARED ? 1 : V;
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const long long b = blockIdx.x / blocks;
+    const ChannelLane ch = channelLane<V, SHARED>(p, int(blockIdx.x % blocks), lane, plan.slots, plan.parts);
     const int n = lengthOf(p, b), span = blockIdx.y;
-    const int begin = span * plan.chunkSteps, end = min(n, begin + plan.chunkSteps);
+    const int begin = span * plan.chunkSteps, end = min(n, begin + plan.chunkSteps), tilesOfSpan = plan.chunkSteps / plan.tile;
     const T* const gp = static_cast<const T*>(p.gate) + b * p.gs[0] + ch.g * p.gs[2];
     const T* const xp = static_cast<const T*>(p.x) + b * p.xs[0] + ch.c * p.xs[2];
     const T* const dp = p.dout ? static_cast<const T*>(p.dout) + b * p.ds[0] + ch.c * p.ds[2] : nullptr;
-    float A = 1.f, U = 0.f, D = 0.f;
-    if (span == 0 && p.h0) U = p.h0[b * p.C + ch.c];
-    __shared__ float4 joined[NW == 1 ? 1 : 2][NW][NW == 1 ? 1 : 64];
+    const BackwardScratch ws = backwardScratch(p, plan);
+    float* const heads = ws.heads + ((b * plan.chunks + span) * tilesOfSpan) * p.C + ch.c;
+    float A[GV], U[V], D[V];
+#pragma unroll
+    for (int v = 0; v < GV; ++v) A[v] = 1.f;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        U[v] = span == 0 && p.h0 ? p.h0[b * p.C + ch.c + v] : 0.f;
+        D[v] = 0.f;
+    }
+    __shared__ float joined[2][NW][GV + 2 * V][64];
     int buffer = 0;
-    for (int tile = begin; tile < end; tile += NW * L) {
-        float a2 = 1.f, u2 = 0.f, d2 = 0.f;
+    for (int tile = begin, j = 0; tile < end; tile += NW * L, ++j) {
+        if (tilesOfSpan > 1 && w == 0 && ch.live) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                heads[(long long)j * p.C + v] = span == 0 ? 0.f : A[SHARED ? 0 : v];
+                heads[ws.headPlane + (long long)j * p.C + v] = U[v];
+            }
+        }
+        const int i0 = tile + w * L;
+        T rawG[L][GV], rawX[L][V], rawD[L][V];
+        loadChannels<T, GV, L>(gp, p.gs[1], i0, n, end, p.reverse, rawG);
+        loadChannels<T, V, L>(xp, p.xs[1], i0, n, end, p.reverse, rawX);
+        if (dp) loadChannels<T, V, L>(dp, p.ds[1], i0, n, end, p.reverse, rawD);
+        float a[L][GV], rest[L][GV], a2[GV], u2[V], d2[V];
+        gatesOf<T, GV, L>(p, rawG, i0, end, a, rest);
+#pragma unroll
+        for (int v = 0; v < V; ++v) u2[v] = d2[v] = 0.f;
+#pragma unroll
+        for (int v = 0; v < GV; ++v) a2[v] = 1.f;
 #pragma unroll
         for (int k = 0; k < L; ++k) {
-            const int i = tile + w * L + k;
-            if (i < end) {
-                const long long t = positionOf(i, n, p.reverse);
-                float a, rest;
-                gateOf<EXP>(toFloat(gp[t * p.gs[1]]), p.scale, a, rest);
-                const float x = toFloat(xp[t * p.xs[1]]);
-                u2 = fmaf(a, u2, BLEND ? rest * x : x);
-                a2 *= a;
-                if (dp) d2 = fmaf(a2, toFloat(dp[t * p.ds[1]]), d2);
-            }
-        }
-        if constexpr (NW > 1) {
-            joined[buffer][w][lane] = make_float4(a2, u2, d2, 0.f);
-            __syncthreads();
 #pragma unroll
-            for (int j = 0; j < NW; ++j) {
-                const float4 s = joined[buffer][j][lane];
-                U = fmaf(s.x, U, s.y);
-                D = fmaf(A, s.z, D);
-                A *= s.x;
+            for (int v = 0; v < GV; ++v) a2[v] *= a[k][v];
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                u2[v] = fmaf(a[k][SHARED ? 0 : v], u2[v], rest[k][SHARED ? 0 : v] * toFloat(rawX[k][v]));
+                if (dp) d2[v] = fmaf(a2[SHARED ? 0 : v], toFloat(rawD[k][v]), d2[v]);
             }
-            buffer ^= 1;
-        } else {
-            U = fmaf(a2, U, u2);
-            D = fmaf(A, d2, D);
-            A *= a2;
         }
+#pragma unroll
+        for (int v = 0; v < GV; ++v) joined[buffer][w][v][lane] = a2[v];
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            joined[buffer][w][GV + v][lane] = u2[v];
+            joined[buffer][w][GV + V + v][lane] = d2[v];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int s = 0; s < NW; ++s) {
+            float as[GV];
+#pragma unroll
+            for (int v = 0; v < GV; ++v) as[v] = joined[buffer][s][v][lane];
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                U[v] = fmaf(as[SHARED ? 0 : v], U[v], joined[buffer][s][GV + v][lane]);
+                D[v] = fmaf(A[SHARED ? 0 : v], joined[buffer][s][GV + V + v][lane], D[v]);
+            }
+#pragma unroll
+            for (int v = 0; v < GV; ++v) A[v] *= as[v];
+        }
+        buffer ^= 1;
     }
     if (w != 0 || !ch.live) return;
-    const long long plane = p.B * plan.chunks * p.C, at = (b * plan.chunks + span) * p.C + ch.c;
-    p.ws[at] = A;
-    p.ws[plane + at] = U;
-    p.ws[2 * plane + at] = D;
+    const long long at = (b * plan.chunks + span) * p.C + ch.c;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        ws.spans[at + v] = A[SHARED ? 0 : v];
+        ws.spans[ws.plane + at + v] = U[v];
+        ws.spans[2 * ws.plane + at + v] = D[v];
+    }
 }
 
-template <class T, bool EXP, bool BLEND, int NW>
+template <class T, int NW, int V, bool SHARED>
 __global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW) void scan_channels_backward_kernel(const ScanParams p, const ScanPlan plan, const int blocks, const long long units) {
-    constexpr int L = kBackwardSteps;
+    constexpr int L = backwardSteps(V), GV = SHARED ? 1 : V;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int w = NW == 1 ? 0 : wave;
     const long long unit = NW == 1 ? blockIdx.x * 4LL + wave : blockIdx.x;
     if (unit >= units) return;
     const long long b = unit / blocks;
-    const ChannelLane ch = channelLane<1>(p, int(unit % blocks), lane, plan.slots, plan.parts);
-    const int n = lengthOf(p, b), span = blockIdx.y;
-    const int begin = span * plan.chunkSteps, end = min(p.T, begin + plan.chunkSteps);
-    const int tiles = (end - begin + plan.tile - 1) / plan.tile;
+    const ChannelLane ch = channelLane<V, SHARED>(p, int(unit % blocks), lane, plan.slots, plan.parts);
+    const int n = lengthOf(p, b), span = gridDim.y - 1 - blockIdx.y;
+    const int begin = span * plan.chunkSteps, end = min(p.T, begin + plan.chunkSteps), inside = min(n, end);
+    const int tiles = (end - begin + plan.tile - 1) / plan.tile, tilesOfSpan = plan.chunkSteps / plan.tile;
     const T* const gp = static_cast<const T*>(p.gate) + b * p.gs[0] + ch.g * p.gs[2];
     const T* const xp = static_cast<const T*>(p.x) + b * p.xs[0] + ch.c * p.xs[2];
     const T* const dp = p.dout ? static_cast<const T*>(p.dout) + b * p.ds[0] + ch.c * p.ds[2] : nullptr;
     T* const dgp = p.dgate ? static_cast<T*>(p.dgate) + b * p.dgs[0] + ch.g * p.dgs[2] : nullptr;
     T* const dxp = p.dx ? static_cast<T*>(p.dx) + b * p.dxs[0] + ch.c * p.dxs[2] : nullptr;
-    const long long plane = plan.chunks > 1 ? p.B * plan.chunks * p.C : 0;
+    const BackwardScratch ws = backwardScratch(p, plan);
     const long long state = b * p.C + ch.c;
-    const int tilesOfSpan = plan.chunkSteps / plan.tile;
-    // the states at the head of every tile, if a span has more than one
     const bool kept = tilesOfSpan > 1;
-    float* const heads = p.ws + 3 * plane + ((b * plan.chunks + span) * tilesOfSpan) * p.C + ch.c;
-    float* const partial = p.ws + 3 * plane + (kept ? p.B * plan.chunks * tilesOfSpan * p.C : 0) + b * p.T * (long long)p.Cg * plan.parts + (long long)ch.g * plan.parts + ch.part;
-    float h = 0.f, k = p.dlast ? p.dlast[state] : 0.f;
-    if (p.h0) h = p.h0[state];
-    if (plan.chunks > 1) {
-        const float* const wa = p.ws + (b * plan.chunks) * p.C + ch.c;
-        if (span > 0) {
-            h = wa[plane];
-            for (int s = 1; s < span; ++s) h = fmaf(wa[(long long)s * p.C], h, wa[plane + (long long)s * p.C]);
-        }
-        for (int s = plan.chunks - 1; s > span; --s) k = fmaf(wa[(long long)s * p.C], k, wa[2 * plane + (long long)s * p.C]);
+    float* const heads = ws.heads + ((b * plan.chunks + span) * tilesOfSpan) * p.C + ch.c;
+    float* const partial = ws.partial + (b * p.T * (long long)p.Cg + ch.g) * plan.parts + ch.part;
+    float h[V], k[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        h[v] = p.h0 ? p.h0[state + v] : 0.f;
+        k[v] = p.dlast ? p.dlast[state + v] : 0.f;
     }
-    __shared__ float4 joined[NW == 1 ? 1 : 2][NW][NW == 1 ? 1 : 64];
+    if (plan.chunks > 1) {
+        const float* const wa = ws.spans + (b * plan.chunks) * p.C + ch.c;
+        if (span > 0) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) h[v] = wa[ws.plane + v];
+#pragma unroll 4
+            for (int s = 1; s < span; ++s)
+#pragma unroll
+                for (int v = 0; v < V; ++v) h[v] = fmaf(wa[(long long)s * p.C + v], h[v], wa[ws.plane + (long long)s * p.C + v]);
+        }
+#pragma unroll 4
+        for (int s = plan.chunks - 1; s > span; --s)
+#pragma unroll
+            for (int v = 0; v < V; ++v) k[v] = fmaf(wa[(long long)s * p.C + v], k[v], wa[2 * ws.plane + (long long)s * p.C + v]);
+    }
+    __shared__ float joined[NW == 1 ? 1 : 2][NW][GV + 3 * V][NW == 1 ? 1 : 64];
     int buffer = 0;
-    if (kept) {
+    if (kept && plan.chunks == 1) {
+        // one span: the states at the head of every tile, for the walk back
+        float at[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) at[v] = h[v];
         for (int j = 0; j < tiles; ++j) {
-            if (w == 0) heads[(long long)j * p.C] = h;  // (written and read again by this lane; dead lanes: the copy of a live one's channel)
-            float a2 = 1.f, u2 = 0.f;
+            if (w == 0)  // (written and read again by this lane; a dead one's channel is a live one's, and so is its value)
+#pragma unroll
+                for (int v = 0; v < V; ++v) heads[(long long)j * p.C + v] = at[v];
+            const int i0 = begin + j * plan.tile + w * L;
+            T rawG[L][GV], rawX[L][V];
+            loadChannels<T, GV, L>(gp, p.gs[1], i0, n, inside, p.reverse, rawG);
+            loadChannels<T, V, L>(xp, p.xs[1], i0, n, inside, p.reverse, rawX);
+            float a[L][GV], rest[L][GV], a2[GV], u2[V];
+            gatesOf<T, GV, L>(p, rawG, i0, inside, a, rest);
+#pragma unroll
+            for (int v = 0; v < V; ++v) u2[v] = NW == 1 ? at[v] : 0.f;
+#pragma unroll
+            for (int v = 0; v < GV; ++v) a2[v] = 1.f;
 #pragma unroll
             for (int q = 0; q < L; ++q) {
-                const int i = begin + j * plan.tile + w * L + q;
-                if (i < n && i < end) {
-                    const long long t = positionOf(i, n, p.reverse);
-                    float a, rest;
-                    gateOf<EXP>(toFloat(gp[t * p.gs[1]]), p.scale, a, rest);
-                    const float x = toFloat(xp[t * p.xs[1]]);
-                    u2 = fmaf(a, u2, BLEND ? rest * x : x);
-                    a2 *= a;
-                }
+#pragma unroll
+                for (int v = 0; v < GV; ++v) a2[v] *= a[q][v];
+#pragma unroll
+                for (int v = 0; v < V; ++v) u2[v] = fmaf(a[q][SHARED ? 0 : v], u2[v], rest[q][SHARED ? 0 : v] * toFloat(rawX[q][v]));
             }
             if constexpr (NW > 1) {
-                joined[buffer][w][lane] = make_float4(a2, u2, 0.f, 0.f);
+#pragma unroll
+                for (int v = 0; v < GV; ++v) joined[buffer][w][v][lane] = a2[v];
+#pragma unroll
+                for (int v = 0; v < V; ++v) joined[buffer][w][GV + v][lane] = u2[v];
                 __syncthreads();
 #pragma unroll
-                for (int s = 0; s < NW; ++s) h = fmaf(joined[buffer][s][lane].x, h, joined[buffer][s][lane].y);
+                for (int s = 0; s < NW; ++s)
+#pragma unroll
+                    for (int v = 0; v < V; ++v) at[v] = fmaf(joined[buffer][s][SHARED ? 0 : v][lane], at[v], joined[buffer][s][GV + v][lane]);
                 buffer ^= 1;
             } else {
-                h = fmaf(a2, h, u2);
+#pragma unroll
+                for (int v = 0; v < V; ++v) at[v] = u2[v];
             }
         }
     }
     for (int j = tiles - 1; j >= 0; --j) {
         const int i0 = begin + j * plan.tile + w * L;
-        float m[L], rest[L], x[L], d[L], before[L];
+        T rawG[L][GV], rawX[L][V], rawD[L][V];
+        loadChannels<T, GV, L>(gp, p.gs[1], i0, n, inside, p.reverse, rawG);
+        loadChannels<T, V, L>(xp, p.xs[1], i0, n, inside, p.reverse, rawX);
+        if (dp) loadChannels<T, V, L>(dp, p.ds[1], i0, n, inside, p.reverse, rawD);
+        // the state at the head of the tile: of a wave on its own its own, of waves that share one what wave 0 says below
+        float head[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            head[v] = h[v];
+            if (kept && w == 0 && begin + j * plan.tile < n)
+                head[v] = plan.chunks == 1 ? heads[(long long)j * p.C + v] : span == 0 ? heads[ws.headPlane + (long long)j * p.C + v]
+                                                                                     : fmaf(heads[(long long)j * p.C + v], h[v], heads[ws.headPlane + (long long)j * p.C + v]);
+        }
+        float a[L][GV], rest[L][GV], x[L][V], d[L][V], a2[GV], u2[V], d2[V];
+        gatesOf<T, GV, L>(p, rawG, i0, inside, a, rest);
+#pragma unroll
+        for (int v = 0; v < V; ++v) u2[v] = d2[v] = 0.f;
+#pragma unroll
+        for (int v = 0; v < GV; ++v) a2[v] = 1.f;
 #pragma unroll
         for (int q = 0; q < L; ++q) {
-            const int i = i0 + q;
-            m[q] = EXP ? 0.f : 1.f;
-            x[q] = d[q] = 0.f;
-            if (i < n && i < end) {
-                const long long t = positionOf(i, n, p.reverse);
-                m[q] = toFloat(gp[t * p.gs[1]]);
-                x[q] = toFloat(xp[t * p.xs[1]]);
-                if (dp) d[q] = toFloat(dp[t * p.ds[1]]);
+#pragma unroll
+            for (int v = 0; v < GV; ++v) a2[v] *= a[q][v];
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                x[q][v] = toFloat(rawX[q][v]);
+                d[q][v] = dp ? toFloat(rawD[q][v]) : 0.f;
+                if (NW > 1) {
+                    u2[v] = fmaf(a[q][SHARED ? 0 : v], u2[v], rest[q][SHARED ? 0 : v] * x[q][v]);
+                    d2[v] = fmaf(a2[SHARED ? 0 : v], d[q][v], d2[v]);
+                }
             }
         }
-        // (the head of the tile: every wave of it needs the state that wave 0 kept)
-        if (kept && NW == 1) h = heads[(long long)j * p.C];
-        float a2 = 1.f, u2 = 0.f, d2 = 0.f;
+        float hw[V], kw[V];
 #pragma unroll
-        for (int q = 0; q < L; ++q) {
-            gateOf<EXP>(m[q], p.scale, m[q], rest[q]);
-            u2 = fmaf(m[q], u2, BLEND ? rest[q] * x[q] : x[q]);
-            a2 *= m[q];
-            d2 = fmaf(a2, d[q], d2);
+        for (int v = 0; v < V; ++v) {
+            hw[v] = head[v];
+            kw[v] = k[v];
         }
-        float hw = h, kw = k;
         if constexpr (NW > 1) {
-            float4 mine = make_float4(a2, u2, d2, 0.f);
-            if (w == 0) mine.w = kept ? heads[(long long)j * p.C] : h;
-            joined[buffer][w][lane] = mine;
+#pragma unroll
+            for (int v = 0; v < GV; ++v) joined[buffer][w][v][lane] = a2[v];
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                joined[buffer][w][GV + v][lane] = u2[v];
+                joined[buffer][w][GV + V + v][lane] = d2[v];
+                if (w == 0) joined[buffer][0][GV + 2 * V + v][lane] = head[v];
+            }
             __syncthreads();
-            hw = joined[buffer][0][lane].w;
+#pragma unroll
+            for (int v = 0; v < V; ++v) hw[v] = joined[buffer][0][GV + 2 * V + v][lane];
 #pragma unroll
             for (int s = 0; s < NW - 1; ++s)
-                if (s < w) hw = fmaf(joined[buffer][s][lane].x, hw, joined[buffer][s][lane].y);
+                if (s < w)
 #pragma unroll
-            for (int s = NW - 1; s >= 0; --s) {
-                if (s == w) kw = k;
-                k = fmaf(joined[buffer][s][lane].x, k, joined[buffer][s][lane].z);
-            }
+                    for (int v = 0; v < V; ++v) hw[v] = fmaf(joined[buffer][s][SHARED ? 0 : v][lane], hw[v], joined[buffer][s][GV + v][lane]);
+#pragma unroll
+            for (int s = NW - 1; s >= 0; --s)
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    if (s == w) kw[v] = k[v];
+                    k[v] = fmaf(joined[buffer][s][SHARED ? 0 : v][lane], k[v], joined[buffer][s][GV + V + v][lane]);
+                }
             buffer ^= 1;
         }
+        float entry[L][V];
 #pragma unroll
-        for (int q = 0; q < L; ++q) {
-            before[q] = hw;
-            hw = fmaf(m[q], hw, BLEND ? rest[q] * x[q] : x[q]);
-        }
+        for (int q = 0; q < L; ++q)
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                entry[q][v] = hw[v];
+                hw[v] = fmaf(a[q][SHARED ? 0 : v], hw[v], rest[q][SHARED ? 0 : v] * x[q][v]);
+            }
 #pragma unroll
         for (int q = L - 1; q >= 0; --q) {
             const int i = i0 + q;
-            const float a = m[q], l = d[q] + kw;
-            const bool in = i < n && i < end;
+            const bool in = i < inside;
             const long long t = positionOf(i, n, p.reverse);
-            if (dxp && i < end && ch.live) dxp[t * p.dxs[1]] = fromFloat<T>(in ? (BLEND ? rest[q] * l : l) : 0.f);
-            if (p.dgate) {
-                float s = l * (BLEND ? before[q] - x[q] : before[q]);
-                if (EXP) s *= p.scale * a;
-                if (plan.slots > 1) {
-                    s = ch.live ? s : 0.f;
-                    for (int o = 1; o < plan.slots; o <<= 1) s += __shfl_xor(s, o, 64);
+            T dx[V], dg[GV];
+            float sum = 0.f;
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                const float av = a[q][SHARED ? 0 : v], l = d[q][v] + kw[v];
+                dx[v] = fromFloat<T>(in ? rest[q][SHARED ? 0 : v] * l : 0.f);
+                float s = l * (p.blend ? entry[q][v] - x[q][v] : entry[q][v]);
+                if (SHARED) {
+                    sum += s;
+                } else {
+                    if (p.exp) s *= p.scale * av;
+                    if (V == 1) sum = s;
+                    else dg[v] = fromFloat<T>(in ? s : 0.f);
                 }
-                const bool first = plan.slots == 1 || (lane & (plan.slots - 1)) == 0;
-                if (i < end && ch.live && first) {
-                    if (plan.parts > 1) partial[t * (long long)p.Cg * plan.parts] = in ? s : 0.f;
-                    else dgp[t * p.dgs[1]] = fromFloat<T>(in ? s : 0.f);
-                }
+                kw[v] = av * l;
             }
-            kw = a * l;
+            if (SHARED) {
+                if (p.exp) sum *= p.scale * a[q][0];
+                dg[0] = fromFloat<T>(in ? sum : 0.f);
+            }
+            bool first = true;
+            if (V == 1) {
+                if (plan.slots > 1) {
+                    sum = ch.live ? sum : 0.f;
+                    for (int o = 1; o < plan.slots; o <<= 1) sum += __shfl_xor(sum, o, 64);
+                    first = (lane & (plan.slots - 1)) == 0;
+                }
+                dg[0] = fromFloat<T>(in ? sum : 0.f);
+            }
+            if (i >= end || !ch.live) continue;
+            if (dxp) storeWide<T, V>(dxp + t * p.dxs[1], dx);
+            if (dgp && first) {
+                if (V == 1 && plan.parts > 1) partial[t * (long long)p.Cg * plan.parts] = in ? sum : 0.f;
+                else storeWide<T, GV>(dgp + t * p.dgs[1], dg);
+            }
         }
-        if constexpr (NW == 1) k = kw;
+        if constexpr (NW == 1) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) k[v] = kw[v];
+        }
     }
-    if (p.dh0 && span == 0 && w == 0 && ch.live) p.dh0[state] = k;
+    if (p.dh0 && span == 0 && w == 0 && ch.live)
+#pragma unroll
+        for (int v = 0; v < V; ++v) p.dh0[state + v] = k[v];
 }
 
 // Sums of the parts of gates with more than 64 channels, in their order.
@@ -449,8 +615,7 @@ __global__ __launch_bounds__(256) void scan_gate_sum_kernel(const ScanParams p, 
 constexpr int kRowSteps = 8;          // steps of a lane, forward
 constexpr int kRowStepsBackward = 4;  // and backward
 
-// Inclusive scan over the `width` lanes of a row: (A, U) of every span from the row's first lane to this one (FORWARD), or (A, U) = (A, D) from this lane to
-// the row's last.
+// (A, U) of this lane's span joined with its row's lanes before it (FORWARD) or behind it, over the `width` lanes of a row: an inclusive scan.
 template <int G, bool FORWARD>
 __device__ __forceinline__ void joinLanes(float& A, float (&U)[G], int width, int lane) {
     const int at = lane & (width - 1);
@@ -467,8 +632,134 @@ __device__ __forceinline__ void joinLanes(float& A, float (&U)[G], int width, in
     }
 }
 
-template <class T, bool EXP, bool BLEND, int G>
-__global__ __launch_bounds__(256) void scan_rows_kernel(const ScanParams p, const int width) {
+// K steps of G channels of one lane, steps i .. i + K - 1 of a sequence of n, with as wide accesses as the strides allow: all of it in one piece, a step in one
+// piece, or element by element.  A lane's steps are 128 bytes of colours with absorption apart from the next lane's: reading them element by element
+// would touch 64 lines with each instruction.
+template <class T, int G, int K>
+struct StepBlock {
+    T v[K * G];  // in the order of memory
+    __device__ __forceinline__ void load(const T* base, long long step, long long channel) {
+        if (channel == 1 && step == G) {
+            loadWide<T, K * G>(v, base);
+        } else if (channel == 1) {
+#pragma unroll
+            for (int q = 0; q < K; ++q) loadWide<T, G>(v + q * G, base + q * step);
+        } else {
+#pragma unroll
+            for (int q = 0; q < K; ++q)
+#pragma unroll
+                for (int c = 0; c < G; ++c) v[q * G + c] = base[q * step + c * channel];
+        }
+    }
+    __device__ __forceinline__ void store(T* base, long long step, long long channel) const {
+        if (channel == 1 && step == G) {
+            storeWide<T, K * G>(base, v);
+        } else if (channel == 1) {
+#pragma unroll
+            for (int q = 0; q < K; ++q) storeWide<T, G>(base + q * step, v + q * G);
+        } else {
+#pragma unroll
+            for (int q = 0; q < K; ++q)
+#pragma unroll
+                for (int c = 0; c < G; ++c) base[q * step + c * channel] = v[q * G + c];
+        }
+    }
+};
+
+// to[q][c] = channel c of step i + q, 0 behind the sequence
+template <class T, int G, int K>
+__device__ __forceinline__ void loadSteps(const T* p, long long step, long long channel, int i, int n, int reverse, float (&to)[K][G]) {
+    if (i + K <= n) {
+        StepBlock<T, G, K> block;
+        if (reverse) {
+            block.load(p + (long long)(n - K - i) * step, step, channel);
+#pragma unroll
+            for (int q = 0; q < K; ++q)
+#pragma unroll
+                for (int c = 0; c < G; ++c) to[q][c] = toFloat(block.v[(K - 1 - q) * G + c]);
+        } else {
+            block.load(p + (long long)i * step, step, channel);
+#pragma unroll
+            for (int q = 0; q < K; ++q)
+#pragma unroll
+                for (int c = 0; c < G; ++c) to[q][c] = toFloat(block.v[q * G + c]);
+        }
+    } else {
+#pragma unroll
+        for (int q = 0; q < K; ++q)
+#pragma unroll
+            for (int c = 0; c < G; ++c) to[q][c] = i + q < n ? toFloat(p[positionOf(i + q, n, reverse) * step + c * channel]) : 0.f;
+    }
+}
+
+// zeros behind the sequence, nothing behind T
+template <class T, int G, int K>
+__device__ __forceinline__ void storeSteps(T* p, long long step, long long channel, int i, int n, int T_, int reverse, const float (&from)[K][G]) {
+    if (i + K <= n) {
+        StepBlock<T, G, K> block;
+        if (reverse) {
+#pragma unroll
+            for (int q = 0; q < K; ++q)
+#pragma unroll
+                for (int c = 0; c < G; ++c) block.v[(K - 1 - q) * G + c] = fromFloat<T>(from[q][c]);
+            block.store(p + (long long)(n - K - i) * step, step, channel);
+        } else {
+#pragma unroll
+            for (int q = 0; q < K; ++q)
+#pragma unroll
+                for (int c = 0; c < G; ++c) block.v[q * G + c] = fromFloat<T>(from[q][c]);
+            block.store(p + (long long)i * step, step, channel);
+        }
+    } else {
+#pragma unroll
+        for (int q = 0; q < K; ++q)
+#pragma unroll
+            for (int c = 0; c < G; ++c)
+                if (i + q < T_) p[positionOf(i + q, n, reverse) * step + c * channel] = fromFloat<T>(i + q < n ? from[q][c] : 0.f);
+    }
+}
+
+// A gate's row with its G channels; `beside`: the gate is the element behind its channels (the colours and absorptions of a transfer function), read with them
+template <class T, int G, int K>
+__device__ __forceinline__ void loadRow(const ScanParams& p, const T* gp, const T* xp, bool beside, int i, int n, float (&g)[K], float (&x)[K][G]) {
+    if (beside) {
+        float both[K][G + 1];
+        loadSteps<T, G + 1, K>(xp, p.xs[1], 1, i, n, p.reverse, both);
+#pragma unroll
+        for (int q = 0; q < K; ++q) {
+            g[q] = both[q][G];
+#pragma unroll
+            for (int c = 0; c < G; ++c) x[q][c] = both[q][c];
+        }
+    } else {
+        float one[K][1];
+        loadSteps<T, 1, K>(gp, p.gs[1], 1, i, n, p.reverse, one);
+#pragma unroll
+        for (int q = 0; q < K; ++q) g[q] = one[q][0];
+        loadSteps<T, G, K>(xp, p.xs[1], G == 1 ? 1 : p.xs[2], i, n, p.reverse, x);
+    }
+}
+
+// a and the factor of x (1 - a of BLEND, 1 of ADD) of a lane's steps; behind the sequence x was read as 0, and the gate is 1
+template <int K>
+__device__ __forceinline__ void rowGates(const ScanParams& p, int i, int n, float (&m)[K], float (&rest)[K]) {
+    if (p.exp) {
+#pragma unroll
+        for (int q = 0; q < K; ++q) gateOf<true>(m[q], p.scale, m[q], rest[q]);
+    } else {
+#pragma unroll
+        for (int q = 0; q < K; ++q) {
+            gateOf<false>(m[q], p.scale, m[q], rest[q]);
+            m[q] = i + q < n ? m[q] : 1.f;
+        }
+    }
+    if (!p.blend)
+#pragma unroll
+        for (int q = 0; q < K; ++q) rest[q] = 1.f;
+}
+
+template <class T, int G>
+__global__ __launch_bounds__(256) void scan_rows_kernel(const ScanParams p, const int width, const bool beside) {
     constexpr int K = kRowSteps;
     const int lane = threadIdx.x & 63, at = lane & (width - 1);
     const long long rows = p.B * p.Cg, own = (blockIdx.x * 4LL + (threadIdx.x >> 6)) * (64 / width) + lane / width;
@@ -485,36 +776,25 @@ __global__ __launch_bounds__(256) void scan_rows_kernel(const ScanParams p, cons
     for (int tile = 0; tile < p.T; tile += width * K) {
         const int i0 = tile + at * K;
         float m[K], u[K][G];
-#pragma unroll
-        for (int q = 0; q < K; ++q) {
-            const int i = i0 + q;
-            m[q] = EXP ? 0.f : 1.f;
-#pragma unroll
-            for (int c = 0; c < G; ++c) u[q][c] = 0.f;
-            if (i < n) {
-                const long long t = positionOf(i, n, p.reverse);
-                m[q] = toFloat(gp[t * p.gs[1]]);
-#pragma unroll
-                for (int c = 0; c < G; ++c) u[q][c] = toFloat(xp[t * p.xs[1] + c * p.xs[2]]);
-            }
-        }
+        loadRow<T, G, K>(p, gp, xp, beside, i0, n, m, u);
         float A = 1.f, U[G];
 #pragma unroll
         for (int c = 0; c < G; ++c) U[c] = 0.f;
+        float rest[K];
+        rowGates<K>(p, i0, n, m, rest);
 #pragma unroll
         for (int q = 0; q < K; ++q) {
-            float rest;
-            gateOf<EXP>(m[q], p.scale, m[q], rest);
 #pragma unroll
             for (int c = 0; c < G; ++c) {
-                if (BLEND) u[q][c] *= rest;
+                u[q][c] *= rest[q];
                 U[c] = fmaf(m[q], U[c], u[q][c]);
             }
             A *= m[q];
         }
         joinLanes<G, true>(A, U, width, lane);
         // the state that enters this lane's span: the row's, taken through the lanes before
-        float before = __shfl_up(A, 1, width), pre[G];
+        const float before = __shfl_up(A, 1, width);
+        float pre[G];
 #pragma unroll
         for (int c = 0; c < G; ++c) {
             const float u1 = __shfl_up(U[c], 1, width);
@@ -523,15 +803,10 @@ __global__ __launch_bounds__(256) void scan_rows_kernel(const ScanParams p, cons
         }
         if (op) {
 #pragma unroll
-            for (int q = 0; q < K; ++q) {
-                const int i = i0 + q;
-                const long long t = positionOf(i, n, p.reverse);
+            for (int q = 0; q < K; ++q)
 #pragma unroll
-                for (int c = 0; c < G; ++c) {
-                    pre[c] = fmaf(m[q], pre[c], u[q][c]);
-                    if (i < p.T && live) op[t * p.os[1] + c * p.os[2]] = fromFloat<T>(i < n ? pre[c] : 0.f);
-                }
-            }
+                for (int c = 0; c < G; ++c) u[q][c] = pre[c] = fmaf(m[q], pre[c], u[q][c]);
+            if (live) storeSteps<T, G, K>(op, p.os[1], G == 1 ? 1 : p.os[2], i0, n, p.T, p.reverse, u);
         }
     }
     if (p.last && live && at == 0)
@@ -539,8 +814,8 @@ __global__ __launch_bounds__(256) void scan_rows_kernel(const ScanParams p, cons
         for (int c = 0; c < G; ++c) p.last[state + c] = h[c];
 }
 
-template <class T, bool EXP, bool BLEND, int G>
-__global__ __launch_bounds__(256) void scan_rows_backward_kernel(const ScanParams p, const int width) {
+template <class T, int G>
+__global__ __launch_bounds__(256) void scan_rows_backward_kernel(const ScanParams p, const int width, const bool beside, const bool outBeside) {
     constexpr int K = kRowStepsBackward;
     const int lane = threadIdx.x & 63, at = lane & (width - 1);
     const long long rows = p.B * p.Cg, own = (blockIdx.x * 4LL + (threadIdx.x >> 6)) * (64 / width) + lane / width;
@@ -580,32 +855,25 @@ __global__ __launch_bounds__(256) void scan_rows_backward_kernel(const ScanParam
                 }
             }
             float m[K], rest[K], x[K][G], d[K][G];
+            loadRow<T, G, K>(p, gp, xp, beside, i0, n, m, x);
+            if (dp && pass) {
+                loadSteps<T, G, K>(dp, p.ds[1], G == 1 ? 1 : p.ds[2], i0, n, p.reverse, d);
+            } else {
 #pragma unroll
-            for (int q = 0; q < K; ++q) {
-                const int i = i0 + q;
-                m[q] = EXP ? 0.f : 1.f;
+                for (int q = 0; q < K; ++q)
 #pragma unroll
-                for (int c = 0; c < G; ++c) x[q][c] = d[q][c] = 0.f;
-                if (i < n) {
-                    const long long t = positionOf(i, n, p.reverse);
-                    m[q] = toFloat(gp[t * p.gs[1]]);
-#pragma unroll
-                    for (int c = 0; c < G; ++c) x[q][c] = toFloat(xp[t * p.xs[1] + c * p.xs[2]]);
-                    if (dp && pass)
-#pragma unroll
-                        for (int c = 0; c < G; ++c) d[q][c] = toFloat(dp[t * p.ds[1] + c * p.ds[2]]);
-                }
+                    for (int c = 0; c < G; ++c) d[q][c] = 0.f;
             }
             float A = 1.f, U[G], D[G];
 #pragma unroll
             for (int c = 0; c < G; ++c) U[c] = D[c] = 0.f;
+            rowGates<K>(p, i0, n, m, rest);
 #pragma unroll
             for (int q = 0; q < K; ++q) {
-                gateOf<EXP>(m[q], p.scale, m[q], rest[q]);
                 A *= m[q];
 #pragma unroll
                 for (int c = 0; c < G; ++c) {
-                    U[c] = fmaf(m[q], U[c], BLEND ? rest[q] * x[q][c] : x[q][c]);
+                    U[c] = fmaf(m[q], U[c], rest[q] * x[q][c]);
                     D[c] = fmaf(A, d[q][c], D[c]);
                 }
             }
@@ -625,7 +893,7 @@ __global__ __launch_bounds__(256) void scan_rows_backward_kernel(const ScanParam
             }
             joinLanes<G, false>(A2, D, width, lane);
             const float behind = __shfl_down(A2, 1, width);
-            float kw[G], state1[K][G];
+            float kw[G], entry[K][G], dg[K][1];
 #pragma unroll
             for (int c = 0; c < G; ++c) {
                 const float d1 = __shfl_down(D[c], 1, width);
@@ -636,30 +904,46 @@ __global__ __launch_bounds__(256) void scan_rows_backward_kernel(const ScanParam
             for (int q = 0; q < K; ++q)
 #pragma unroll
                 for (int c = 0; c < G; ++c) {
-                    state1[q][c] = pre[c];
-                    pre[c] = fmaf(m[q], pre[c], BLEND ? rest[q] * x[q][c] : x[q][c]);
+                    entry[q][c] = pre[c];
+                    pre[c] = fmaf(m[q], pre[c], rest[q] * x[q][c]);
                 }
 #pragma unroll
             for (int q = K - 1; q >= 0; --q) {
-                const int i = i0 + q;
-                const long long t = positionOf(i, n, p.reverse);
-                const float a = m[q];
                 float s = 0.f;
 #pragma unroll
                 for (int c = 0; c < G; ++c) {
                     const float l = d[q][c] + kw[c];
-                    s = fmaf(l, BLEND ? state1[q][c] - x[q][c] : state1[q][c], s);
-                    if (dxp && i < p.T && live) dxp[t * p.dxs[1] + c * p.dxs[2]] = fromFloat<T>(i < n ? (BLEND ? rest[q] * l : l) : 0.f);
-                    kw[c] = a * l;
+                    s = fmaf(l, p.blend ? entry[q][c] - x[q][c] : entry[q][c], s);
+                    x[q][c] = rest[q] * l;
+                    kw[c] = m[q] * l;
                 }
-                if (EXP) s *= p.scale * a;
-                if (dgp && i < p.T && live) dgp[t * p.dgs[1]] = fromFloat<T>(i < n ? s : 0.f);
+                dg[q][0] = p.exp ? s * (p.scale * m[q]) : s;
+            }
+            if (!live) continue;
+            if (outBeside) {
+                float both[K][G + 1];
+#pragma unroll
+                for (int q = 0; q < K; ++q) {
+                    both[q][G] = dg[q][0];
+#pragma unroll
+                    for (int c = 0; c < G; ++c) both[q][c] = x[q][c];
+                }
+                storeSteps<T, G + 1, K>(dxp, p.dxs[1], 1, i0, n, p.T, p.reverse, both);
+            } else {
+                if (dgp) storeSteps<T, 1, K>(dgp, p.dgs[1], 1, i0, n, p.T, p.reverse, dg);
+                if (dxp) storeSteps<T, G, K>(dxp, p.dxs[1], G == 1 ? 1 : p.dxs[2], i0, n, p.T, p.reverse, x);
             }
         }
     }
     if (p.dh0 && live && at == 0)
 #pragma unroll
         for (int c = 0; c < G; ++c) p.dh0[state + c] = k[c];
+}
+
+// The gate is the element behind its row's channels: one tensor of colours and absorptions, or its gradient
+bool gateBeside(const void* x, const long long* xs, const void* gate, const long long* gs, const ScanParams& p, size_t e) {
+    return p.Cg == 1 && (p.G == 1 || xs[2] == 1) && xs[1] == gs[1] && (xs[0] == gs[0] || p.B == 1) && (p.T == 1 || xs[1] > p.G) &&
+           static_cast<const char*>(gate) == static_cast<const char*>(x) + p.G * e;
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -673,14 +957,10 @@ int powerOfTwoAtLeast(long long v) {
 }
 
 template <class F>
-hipError_t withTypes(int dtype, int gateMode, int inputMode, F&& f) {
-    auto modes = [&](auto element) {
-        if (gateMode == FVSRN_GATE_EXP) return inputMode == FVSRN_INPUT_BLEND ? f(element, std::true_type{}, std::true_type{}) : f(element, std::true_type{}, std::false_type{});
-        return inputMode == FVSRN_INPUT_BLEND ? f(element, std::false_type{}, std::true_type{}) : f(element, std::false_type{}, std::false_type{});
-    };
-    if (dtype == FVSRN_TENSOR_F16) return modes(f16_t{});
-    if (dtype == FVSRN_TENSOR_BF16) return modes(bf16_t{});
-    return modes(float{});
+hipError_t withType(int dtype, F&& f) {
+    if (dtype == FVSRN_TENSOR_F16) return f(f16_t{});
+    if (dtype == FVSRN_TENSOR_BF16) return f(bf16_t{});
+    return f(float{});
 }
 
 template <class F>
@@ -691,6 +971,23 @@ hipError_t withGroup(int G, F&& f) {
         case 3: return f(std::integral_constant<int, 3>{});
         default: return f(std::integral_constant<int, 4>{});
     }
+}
+
+// channels of a lane with gates of their own: 8 bytes, and half of it backwards, where a step has twice the registers
+constexpr int widestLane(int elementBytes, bool backward) { return elementBytes == 2 && !backward ? 4 : 2; }
+
+// f(channels of a lane, whether they share a gate)
+template <class T, bool BACKWARD, class F>
+hipError_t withLane(const ScanPlan& plan, F&& f) {
+    if (plan.shared) {
+        if (plan.vec == 2) return f(std::integral_constant<int, 2>{}, std::true_type{});
+        if (plan.vec == 3) return f(std::integral_constant<int, 3>{}, std::true_type{});
+        return f(std::integral_constant<int, 4>{}, std::true_type{});
+    }
+    if constexpr (widestLane(sizeof(T), BACKWARD) == 4)
+        if (plan.vec == 4) return f(std::integral_constant<int, 4>{}, std::false_type{});
+    if (plan.vec == 2) return f(std::integral_constant<int, 2>{}, std::false_type{});
+    return f(std::integral_constant<int, 1>{}, std::false_type{});
 }
 
 }  // namespace
@@ -711,12 +1008,24 @@ ScanPlan planScan(const ScanParams& p, int dtype, bool backward) {
         plan.wsFloats = backward && tiles > 1 ? size_t(p.B) * p.C * tiles : 0;
         return plan;
     }
-    const int L = backward ? kBackwardSteps : kForwardSteps;
-    if (backward && p.G > 1) {
+    // Channels of a lane.  A gate's two to four, if they are adjacent: its factor is worked out once and its gradient summed in the lane.  Otherwise
+    // adjacent channels with adjacent gates, for 8 bytes a load where that leaves every lane something to do.
+    // (The strides of operands that are not there count too: the scratch memory is asked for before the pointers are known.)
+    const bool adjacent = p.xs[2] == 1 && (backward ? p.ds[2] == 1 && p.dxs[2] == 1 : p.os[2] == 1);
+    if (adjacent && p.G >= 2 && p.G <= 4) {
+        plan.vec = p.G;
+        plan.shared = 1;
+    } else if (adjacent && p.G == 1 && p.gs[2] == 1 && (!backward || p.dgs[2] == 1)) {
+        const int most = widestLane(dtype == FVSRN_TENSOR_F32 ? 4 : 2, backward);
+        for (int v = most; v > 1 && plan.vec == 1; v >>= 1)
+            if (p.C % v == 0 && p.C >= 64 * v) plan.vec = v;
+    }
+    const int L = backward ? backwardSteps(plan.vec) : forwardSteps(plan.vec);
+    if (backward && p.G > 1 && !plan.shared) {
         plan.slots = std::min(64, powerOfTwoAtLeast(p.G));
         plan.parts = (p.G + 63) / 64;
     }
-    const long long units = p.B * channelBlocks(p, plan.vec, plan.slots, plan.parts);
+    const long long units = p.B * channelBlocks(p, plan);
     // Waves share a tile of steps while there are fewer than 16 waves of channels for each of the 256 CUs.
     plan.waves = units >= 4096 || p.T <= 2 * L ? 1 : kScanWaves;
     plan.tile = plan.waves * L;
@@ -724,74 +1033,74 @@ ScanPlan planScan(const ScanParams& p, int dtype, bool backward) {
     // Spans: two workgroups for each CU, and at least two tiles a span.
     const long long want = plan.waves == 1 ? 1 : (512 + units - 1) / units;
     const int spans = int(std::max(1LL, std::min(want, (long long)tiles / 2)));
-    const int tilesOfSpan = (tiles + spans - 1) / std::max(1, spans);
-    plan.chunks = std::max(1, (tiles + tilesOfSpan - 1) / std::max(1, tilesOfSpan));
-    plan.chunkSteps = std::max(1, tilesOfSpan) * plan.tile;
-    const size_t state = size_t(p.B) * p.C;
-    if (!backward) {
-        plan.wsFloats = plan.chunks > 1 ? 2 * state * plan.chunks : 0;
-    } else {
-        plan.wsFloats = plan.chunks > 1 ? 3 * state * plan.chunks : 0;
-        if (tilesOfSpan > 1) plan.wsFloats += state * plan.chunks * tilesOfSpan;
-        if (plan.parts > 1) plan.wsFloats += size_t(p.B) * p.T * p.Cg * plan.parts;
-    }
+    const int tilesOfSpan = std::max(1, (tiles + spans - 1) / spans);
+    plan.chunks = std::max(1, (tiles + tilesOfSpan - 1) / tilesOfSpan);
+    plan.chunkSteps = tilesOfSpan * plan.tile;
+    plan.wsFloats = backward ? backwardFloats(p, plan) : plan.chunks > 1 ? 2 * size_t(p.B) * p.C * plan.chunks : 0;
     return plan;
 }
 
-hipError_t launch_gated_scan(const ScanParams& p, const ScanPlan& plan, int dtype, int gateMode, int inputMode, hipStream_t s) {
-    return withTypes(dtype, gateMode, inputMode, [&](auto element, auto isExp, auto isBlend) {
+hipError_t launch_gated_scan(const ScanParams& p, const ScanPlan& plan, int dtype, hipStream_t s) {
+    return withType(dtype, [&](auto element) {
         typedef decltype(element) T;
-        constexpr bool EXP = decltype(isExp)::value, BLEND = decltype(isBlend)::value;
         if (plan.rows) {
             const unsigned grid = unsigned((p.B * p.Cg * plan.width + 255) / 256);
             return withGroup(p.G, [&](auto g) {
-                scan_rows_kernel<T, EXP, BLEND, decltype(g)::value><<<grid, 256, 0, s>>>(p, plan.width);
+                scan_rows_kernel<T, decltype(g)::value><<<grid, 256, 0, s>>>(p, plan.width, gateBeside(p.x, p.xs, p.gate, p.gs, p, sizeof(T)));
                 return hipGetLastError();
             });
         }
-        const int blocks = int(channelBlocks(p, plan.vec, 1, 1));
+        const int blocks = int(channelBlocks(p, plan));
         const long long units = p.B * blocks;
-        if (plan.waves == 1) {
-            scan_channels_kernel<T, EXP, BLEND, 1, 1, false><<<unsigned((units + 3) / 4), 256, 0, s>>>(p, plan, blocks, units);
+        return withLane<T, false>(plan, [&](auto vec, auto shared) {
+            constexpr int V = decltype(vec)::value;
+            constexpr bool SHARED = decltype(shared)::value;
+            if (plan.waves == 1) {
+                scan_channels_kernel<T, 1, V, SHARED, false><<<unsigned((units + 3) / 4), 256, 0, s>>>(p, plan, blocks, units);
+                return hipGetLastError();
+            }
+            const dim3 grid(unsigned(units), unsigned(plan.chunks));
+            if (plan.chunks > 1) {
+                scan_channels_kernel<T, kScanWaves, V, SHARED, true><<<grid, 64 * kScanWaves, 0, s>>>(p, plan, blocks, units);
+                if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+            }
+            scan_channels_kernel<T, kScanWaves, V, SHARED, false><<<grid, 64 * kScanWaves, 0, s>>>(p, plan, blocks, units);
             return hipGetLastError();
-        }
-        const dim3 grid(unsigned(units), unsigned(plan.chunks));
-        if (plan.chunks > 1) {
-            scan_channels_kernel<T, EXP, BLEND, kScanWaves, 1, true><<<grid, 64 * kScanWaves, 0, s>>>(p, plan, blocks, units);
-            if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
-        }
-        scan_channels_kernel<T, EXP, BLEND, kScanWaves, 1, false><<<grid, 64 * kScanWaves, 0, s>>>(p, plan, blocks, units);
-        return hipGetLastError();
+        });
     });
 }
 
-hipError_t launch_gated_scan_backward(const ScanParams& p, const ScanPlan& plan, int dtype, int gateMode, int inputMode, hipStream_t s) {
-    return withTypes(dtype, gateMode, inputMode, [&](auto element, auto isExp, auto isBlend) {
+hipError_t launch_gated_scan_backward(const ScanParams& p, const ScanPlan& plan, int dtype, hipStream_t s) {
+    return withType(dtype, [&](auto element) {
         typedef decltype(element) T;
-        constexpr bool EXP = decltype(isExp)::value, BLEND = decltype(isBlend)::value;
         if (plan.rows) {
             const unsigned grid = unsigned((p.B * p.Cg * plan.width + 255) / 256);
             return withGroup(p.G, [&](auto g) {
-                scan_rows_backward_kernel<T, EXP, BLEND, decltype(g)::value><<<grid, 256, 0, s>>>(p, plan.width);
+                scan_rows_backward_kernel<T, decltype(g)::value><<<grid, 256, 0, s>>>(
+                    p, plan.width, gateBeside(p.x, p.xs, p.gate, p.gs, p, sizeof(T)), p.dx && p.dgate && gateBeside(p.dx, p.dxs, p.dgate, p.dgs, p, sizeof(T)));
                 return hipGetLastError();
             });
         }
-        const int blocks = int(channelBlocks(p, 1, plan.slots, plan.parts));
+        const int blocks = int(channelBlocks(p, plan));
         const long long units = p.B * blocks;
-        if (plan.waves == 1) {
-            scan_channels_backward_kernel<T, EXP, BLEND, 1><<<unsigned((units + 3) / 4), 256, 0, s>>>(p, plan, blocks, units);
-        } else {
+        const hipError_t e = withLane<T, true>(plan, [&](auto vec, auto shared) {
+            constexpr int V = decltype(vec)::value;
+            constexpr bool SHARED = decltype(shared)::value;
+            if (plan.waves == 1) {
+                scan_channels_backward_kernel<T, 1, V, SHARED><<<unsigned((units + 3) / 4), 256, 0, s>>>(p, plan, blocks, units);
+                return hipGetLastError();
+            }
             const dim3 grid(unsigned(units), unsigned(plan.chunks));
             if (plan.chunks > 1) {
-                scan_channels_spans_kernel<T, EXP, BLEND, kScanWaves><<<grid, 64 * kScanWaves, 0, s>>>(p, plan, blocks, units);
+                scan_channels_spans_kernel<T, kScanWaves, V, SHARED><<<grid, 64 * kScanWaves, 0, s>>>(p, plan, blocks);
                 if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
             }
-            scan_channels_backward_kernel<T, EXP, BLEND, kScanWaves><<<grid, 64 * kScanWaves, 0, s>>>(p, plan, blocks, units);
-        }
-        if (const hipError_t e = hipGetLastError(); e != hipSuccess || plan.parts == 1 || !p.dgate) return e;
+            scan_channels_backward_kernel<T, kScanWaves, V, SHARED><<<grid, 64 * kScanWaves, 0, s>>>(p, plan, blocks, units);
+            return hipGetLastError();
+        });
+        if (e != hipSuccess || plan.parts == 1 || !p.dgate) return e;
         const long long count = p.B * p.T * (long long)p.Cg;
-        const float* const partial = p.ws + plan.wsFloats - size_t(count) * plan.parts;
-        scan_gate_sum_kernel<T><<<unsigned(std::min(4096LL, (count + 255) / 256)), 256, 0, s>>>(p, partial, plan.parts);
+        scan_gate_sum_kernel<T><<<unsigned(std::min(4096LL, (count + 255) / 256)), 256, 0, s>>>(p, backwardScratch(p, plan).partial, plan.parts);
         return hipGetLastError();
     });
 }

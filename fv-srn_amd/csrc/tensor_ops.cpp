@@ -102,6 +102,8 @@ int scanShape(ScanCall& c, bool backward) {
     p.G = p.Cg ? p.C / p.Cg : 1;
     p.scale = d.gate_scale;
     p.reverse = d.reverse != 0;
+    p.exp = d.gate_mode == FVSRN_GATE_EXP;
+    p.blend = d.input_mode == FVSRN_INPUT_BLEND;
     for (int i = 0; i < 3; ++i) {
         p.gs[i] = d.gate_stride[i]; p.xs[i] = d.x_stride[i]; p.os[i] = d.out_stride[i];
         p.ds[i] = d.dout_stride[i]; p.dgs[i] = d.dgate_stride[i]; p.dxs[i] = d.dx_stride[i];
@@ -165,7 +167,7 @@ int fvsrn_gated_scan(const fvsrn_scan_desc* desc, const void* d_gate, const void
         if (fvsrn_device_count() == 0) return noDevice();
         p.gate = d_gate; p.x = d_x; p.h0 = d_h0; p.lengths = d_lengths; p.out = d_out; p.last = d_last;
         p.ws = static_cast<float*>(d_workspace);
-        const hipError_t err = launch_gated_scan(p, c.plan, desc->dtype, desc->gate_mode, desc->input_mode, static_cast<hipStream_t>(stream));
+        const hipError_t err = launch_gated_scan(p, c.plan, desc->dtype, static_cast<hipStream_t>(stream));
         if (err != hipSuccess) return fail(FVSRN_ERR_DEVICE, std::string("gated_scan failed: ") + hipGetErrorString(err));
         return FVSRN_OK;
     });
@@ -207,7 +209,7 @@ int fvsrn_gated_scan_backward(const fvsrn_scan_desc* desc, const void* d_gate, c
         p.gate = d_gate; p.x = d_x; p.h0 = d_h0; p.lengths = d_lengths; p.dout = d_dout; p.dlast = d_dlast;
         p.dgate = d_dgate; p.dx = d_dx; p.dh0 = d_dh0;
         p.ws = static_cast<float*>(d_workspace);
-        const hipError_t err = launch_gated_scan_backward(p, c.plan, desc->dtype, desc->gate_mode, desc->input_mode, static_cast<hipStream_t>(stream));
+        const hipError_t err = launch_gated_scan_backward(p, c.plan, desc->dtype, static_cast<hipStream_t>(stream));
         if (err != hipSuccess) return fail(FVSRN_ERR_DEVICE, std::string("gated_scan_backward failed: ") + hipGetErrorString(err));
         return FVSRN_OK;
     });

@@ -17,7 +17,7 @@ struct ScanParams {
     long long B;
     int T, C, Cg, G;  // steps, channels, gate channels, channels of a gate
     float scale;
-    int reverse;
+    int reverse, exp, blend;  // exp: FVSRN_GATE_EXP; blend: FVSRN_INPUT_BLEND
 };
 
 // How a call is cut (planScan): `rows` lays the lanes along the steps of one gate (few channels beside each other), otherwise lanes are channels.
@@ -26,6 +26,7 @@ struct ScanPlan {
     int width;       // rows: lanes of a wave that share a row
     int waves;       // channels: waves that share a tile of steps (1 or kScanWaves)
     int vec;         // channels: adjacent channels of a lane
+    int shared;      // channels: those of a lane have one gate
     int tile;        // steps of a tile
     int chunks;      // spans of steps that run side by side
     int chunkSteps;  // steps of a span, a multiple of the tile
@@ -34,8 +35,8 @@ struct ScanPlan {
     size_t wsFloats; // scratch memory
 };
 ScanPlan planScan(const ScanParams& p, int dtype, bool backward);
-hipError_t launch_gated_scan(const ScanParams& p, const ScanPlan& plan, int dtype, int gateMode, int inputMode, hipStream_t s);
-hipError_t launch_gated_scan_backward(const ScanParams& p, const ScanPlan& plan, int dtype, int gateMode, int inputMode, hipStream_t s);
+hipError_t launch_gated_scan(const ScanParams& p, const ScanPlan& plan, int dtype, hipStream_t s);
+hipError_t launch_gated_scan_backward(const ScanParams& p, const ScanPlan& plan, int dtype, hipStream_t s);
 
 struct QuantizeParams {
     const void* x;

@@ -518,7 +518,8 @@ int fvsrn_matmul_int8(const signed char* d_a, long long lda, const float* d_scal
  * of a magnitude over 1 can overflow there although the recurrence itself would not.
  * d_lengths (int32 per batch element, clamped to 0 .. length; NULL: all `length`): behind a sequence's length nothing is read, and outputs and
  * gradients there are written as zero.  The state is held in 32 bits whatever the dtype; h0 and last are [batch][channels] floats.
- * Inputs may have any strides, zero and negative ones too (broadcast inputs; their gradients come per element); outputs may not overlap themselves. */
+ * Inputs may have any strides, zero and negative ones too (broadcast inputs; their gradients come per element); outputs may not overlap themselves.
+ * The strides of an operand that is NULL make no address, but its channel stride takes part in the choice of a kernel (and of the scratch memory): leave it 1. */
 typedef enum { FVSRN_GATE_VALUE = 0, FVSRN_GATE_EXP = 1 } fvsrn_gate_mode;
 typedef enum { FVSRN_INPUT_ADD = 0, FVSRN_INPUT_BLEND = 1 } fvsrn_input_mode;
 typedef struct {
@@ -529,7 +530,7 @@ typedef struct {
     int length;                       /* steps T                                                                        */
     long long batch, channels, gate_channels; /* gate_channels divides channels                                         */
     long long gate_stride[3], x_stride[3];    /* batch, step, channel; gate is [batch][T][gate_channels], x [batch][T][channels] */
-    long long out_stride[3];          /* states, and ignored without them                                               */
+    long long out_stride[3];          /* states                                                                         */
     long long dout_stride[3], dgate_stride[3], dx_stride[3]; /* backward only                                           */
 } fvsrn_scan_desc;
 size_t fvsrn_scan_desc_size(void);
