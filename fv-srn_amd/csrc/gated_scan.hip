@@ -612,8 +612,7 @@ __global__ __launch_bounds__(256) void scan_gate_sum_kernel(const ScanParams p, 
 // lanes are steps
 // ---------------------------------------------------------------------------------------------------------------------
 
-constexpr int kRowSteps = 8;          // steps of a lane, forward
-constexpr int kRowStepsBackward = 4;  // and backward
+constexpr int kRowSteps = 8;  // steps of a lane
 
 // (A, U) of this lane's span joined with its row's lanes before it (FORWARD) or behind it, over the `width` lanes of a row: an inclusive scan.
 template <int G, bool FORWARD>
@@ -758,30 +757,133 @@ __device__ __forceinline__ void rowGates(const ScanParams& p, int i, int n, floa
         for (int q = 0; q < K; ++q) rest[q] = 1.f;
 }
 
+// Scratch memory of rows that are cut into spans: for each span A (0 for span 0, whose U starts from h0), U and, backward, D of the G channels; each row's h0;
+// backward, the state at the head of each tile.
+struct RowScratch {
+    float *spans, *h0, *heads;
+};
+__host__ __device__ inline RowScratch rowScratch(const ScanParams& p, const ScanPlan& plan, bool backward) {
+    RowScratch r;
+    const long long rows = plan.chunks > 1 ? p.B * p.Cg : 0;
+    r.spans = p.ws;
+    r.h0 = r.spans + rows * plan.chunks * (1 + (backward ? 2 : 1) * p.G);
+    r.heads = r.h0 + rows * p.G;
+    return r;
+}
+
+// What spans from .. to - 1 of a row make of what enters them: (A, U) in all lanes, U from h before them, or (A, D), D from k behind them.  64 lanes take a part each.
+template <int G, bool FORWARD>
+__device__ __forceinline__ void foldSpans(const float* spans, int entry, int from, int to, int lane, float& A, float (&U)[G]) {
+    const int each = (to - from + 63) / 64;
+    const int first = min(to, from + lane * each), last = min(to, first + each);
+    A = 1.f;
+#pragma unroll
+    for (int c = 0; c < G; ++c) U[c] = 0.f;
+    for (int s = first; s < last; ++s) {
+        const float* const e = spans + (long long)s * entry;
+        const float a = e[0];
+#pragma unroll
+        for (int c = 0; c < G; ++c) U[c] = FORWARD ? fmaf(a, U[c], e[1 + c]) : fmaf(A, e[1 + G + c], U[c]);
+        A *= a;
+    }
+    joinLanes<G, FORWARD>(A, U, 64, lane);
+    A = __shfl(A, FORWARD ? 63 : 0, 64);
+#pragma unroll
+    for (int c = 0; c < G; ++c) U[c] = __shfl(U[c], FORWARD ? 63 : 0, 64);
+}
+
+// First launch of a call whose rows are cut into spans (few rows with many steps): a wave per row and span
+template <class T, int G, bool BACKWARD>
+__global__ __launch_bounds__(256) void scan_rows_spans_kernel(const ScanParams p, const ScanPlan plan, const bool beside) {
+    constexpr int K = kRowSteps, ENTRY = 1 + (BACKWARD ? 2 : 1) * G;
+    const int lane = threadIdx.x & 63, span = blockIdx.y;
+    const long long rows = p.B * p.Cg, row = blockIdx.x * 4LL + (threadIdx.x >> 6);
+    if (row >= rows) return;
+    const long long b = row / p.Cg, g = row % p.Cg;
+    const int n = lengthOf(p, b), begin = span * plan.chunkSteps, end = min(n, begin + plan.chunkSteps);
+    const T* const gp = static_cast<const T*>(p.gate) + b * p.gs[0] + g * p.gs[2];
+    const T* const xp = static_cast<const T*>(p.x) + b * p.xs[0] + g * G * p.xs[2];
+    const T* const dp = BACKWARD && p.dout ? static_cast<const T*>(p.dout) + b * p.ds[0] + g * G * p.ds[2] : nullptr;
+    const RowScratch ws = rowScratch(p, plan, BACKWARD);
+    float At = 1.f, Ut[G], Dt[G];
+#pragma unroll
+    for (int c = 0; c < G; ++c) {
+        Ut[c] = span == 0 && p.h0 ? p.h0[b * p.C + g * G + c] : 0.f;
+        Dt[c] = 0.f;
+        if (span == 0 && lane == 0) ws.h0[row * G + c] = Ut[c];
+    }
+    for (int tile = begin; tile < end; tile += 64 * K) {
+        const int i0 = tile + lane * K;
+        float m[K], rest[K], x[K][G], d[K][G];
+        loadRow<T, G, K>(p, gp, xp, beside, i0, n, m, x);
+        if (dp) loadSteps<T, G, K>(dp, p.ds[1], G == 1 ? 1 : p.ds[2], i0, n, p.reverse, d);
+        rowGates<K>(p, i0, n, m, rest);
+        float A = 1.f, U[G], D[G];
+#pragma unroll
+        for (int c = 0; c < G; ++c) U[c] = D[c] = 0.f;
+#pragma unroll
+        for (int q = 0; q < K; ++q) {
+            A *= m[q];
+#pragma unroll
+            for (int c = 0; c < G; ++c) {
+                U[c] = fmaf(m[q], U[c], rest[q] * x[q][c]);
+                if (dp) D[c] = fmaf(A, d[q][c], D[c]);
+            }
+        }
+        float A2 = A;
+        joinLanes<G, true>(A, U, 64, lane);
+        A = __shfl(A, 63, 64);
+        if (dp) joinLanes<G, false>(A2, D, 64, lane);
+#pragma unroll
+        for (int c = 0; c < G; ++c) {
+            Ut[c] = fmaf(A, Ut[c], __shfl(U[c], 63, 64));
+            if (dp) Dt[c] = fmaf(At, __shfl(D[c], 0, 64), Dt[c]);
+        }
+        At *= A;
+    }
+    if (lane != 0) return;
+    float* const e = ws.spans + (row * plan.chunks + span) * ENTRY;
+    e[0] = span == 0 ? 0.f : At;
+#pragma unroll
+    for (int c = 0; c < G; ++c) {
+        e[1 + c] = Ut[c];
+        if (BACKWARD) e[1 + G + c] = Dt[c];
+    }
+}
+
 template <class T, int G>
-__global__ __launch_bounds__(256) void scan_rows_kernel(const ScanParams p, const int width, const bool beside) {
+__global__ __launch_bounds__(256) void scan_rows_kernel(const ScanParams p, const ScanPlan plan, const bool beside) {
     constexpr int K = kRowSteps;
-    const int lane = threadIdx.x & 63, at = lane & (width - 1);
+    const int width = plan.width, lane = threadIdx.x & 63, at = lane & (width - 1), span = blockIdx.y;
     const long long rows = p.B * p.Cg, own = (blockIdx.x * 4LL + (threadIdx.x >> 6)) * (64 / width) + lane / width;
     const bool live = own < rows;
     const long long row = live ? own : rows - 1, b = row / p.Cg, g = row % p.Cg;
-    const int n = lengthOf(p, b);
+    // (a row with more than one tile has a wave for itself: only then the loop below ends at its own length)
+    const int n = lengthOf(p, b), begin = span * plan.chunkSteps, end = min(p.out || width < 64 ? p.T : n, begin + plan.chunkSteps);
     const T* const gp = static_cast<const T*>(p.gate) + b * p.gs[0] + g * p.gs[2];
     const T* const xp = static_cast<const T*>(p.x) + b * p.xs[0] + g * G * p.xs[2];
     T* const op = p.out ? static_cast<T*>(p.out) + b * p.os[0] + g * G * p.os[2] : nullptr;
     const long long state = b * p.C + g * G;
     float h[G];
+    if (plan.chunks > 1) {
+        const RowScratch ws = rowScratch(p, plan, false);
+        float A;
+        if (span > 0) foldSpans<G, true>(ws.spans + row * plan.chunks * (1 + G), 1 + G, 0, span, lane, A, h);
+        else
 #pragma unroll
-    for (int c = 0; c < G; ++c) h[c] = p.h0 ? p.h0[state + c] : 0.f;
-    for (int tile = 0; tile < p.T; tile += width * K) {
+            for (int c = 0; c < G; ++c) h[c] = ws.h0[row * G + c];  // (a copy: d_last may be d_h0)
+    } else {
+#pragma unroll
+        for (int c = 0; c < G; ++c) h[c] = p.h0 ? p.h0[state + c] : 0.f;
+    }
+    for (int tile = begin; tile < end; tile += width * K) {
         const int i0 = tile + at * K;
-        float m[K], u[K][G];
+        float m[K], rest[K], u[K][G];
         loadRow<T, G, K>(p, gp, xp, beside, i0, n, m, u);
+        rowGates<K>(p, i0, n, m, rest);
         float A = 1.f, U[G];
 #pragma unroll
         for (int c = 0; c < G; ++c) U[c] = 0.f;
-        float rest[K];
-        rowGates<K>(p, i0, n, m, rest);
 #pragma unroll
         for (int q = 0; q < K; ++q) {
 #pragma unroll
@@ -809,15 +911,15 @@ __global__ __launch_bounds__(256) void scan_rows_kernel(const ScanParams p, cons
             if (live) storeSteps<T, G, K>(op, p.os[1], G == 1 ? 1 : p.os[2], i0, n, p.T, p.reverse, u);
         }
     }
-    if (p.last && live && at == 0)
+    if (p.last && live && at == 0 && span == plan.chunks - 1)
 #pragma unroll
         for (int c = 0; c < G; ++c) p.last[state + c] = h[c];
 }
 
 template <class T, int G>
-__global__ __launch_bounds__(256) void scan_rows_backward_kernel(const ScanParams p, const int width, const bool beside, const bool outBeside) {
-    constexpr int K = kRowStepsBackward;
-    const int lane = threadIdx.x & 63, at = lane & (width - 1);
+__global__ __launch_bounds__(256) void scan_rows_backward_kernel(const ScanParams p, const ScanPlan plan, const bool beside, const bool outBeside) {
+    constexpr int K = kRowSteps;
+    const int width = plan.width, lane = threadIdx.x & 63, at = lane & (width - 1), span = blockIdx.y;
     const long long rows = p.B * p.Cg, own = (blockIdx.x * 4LL + (threadIdx.x >> 6)) * (64 / width) + lane / width;
     const bool live = own < rows;
     const long long row = live ? own : rows - 1, b = row / p.Cg, g = row % p.Cg;
@@ -828,18 +930,28 @@ __global__ __launch_bounds__(256) void scan_rows_backward_kernel(const ScanParam
     T* const dgp = p.dgate ? static_cast<T*>(p.dgate) + b * p.dgs[0] + g * p.dgs[2] : nullptr;
     T* const dxp = p.dx ? static_cast<T*>(p.dx) + b * p.dxs[0] + g * G * p.dxs[2] : nullptr;
     const long long state = b * p.C + g * G;
-    const int tile = width * K, tiles = (p.T + tile - 1) / tile;
-    float* const heads = p.ws + row * tiles * G;  // the row's state at the head of each tile, if there is more than one
+    const int tile = width * K, tilesOfSpan = (plan.chunkSteps + tile - 1) / tile;
+    const int firstTile = span * tilesOfSpan, tiles = min(tilesOfSpan, (p.T + tile - 1) / tile - firstTile);
+    const RowScratch ws = rowScratch(p, plan, true);
+    float* const heads = ws.heads + (row * plan.chunks + span) * tilesOfSpan * G;  // the row's state at the head of each tile of the span, if there is more than one
     float h[G], k[G];
 #pragma unroll
     for (int c = 0; c < G; ++c) {
         h[c] = p.h0 ? p.h0[state + c] : 0.f;
         k[c] = p.dlast ? p.dlast[state + c] : 0.f;
     }
+    if (plan.chunks > 1) {
+        const float* const spans = ws.spans + row * plan.chunks * (1 + 2 * G);
+        float A, D[G];
+        if (span > 0) foldSpans<G, true>(spans, 1 + 2 * G, 0, span, lane, A, h);
+        foldSpans<G, false>(spans, 1 + 2 * G, span + 1, plan.chunks, lane, A, D);
+#pragma unroll
+        for (int c = 0; c < G; ++c) k[c] = fmaf(A, k[c], D[c]);
+    }
     for (int pass = tiles > 1 ? 0 : 1; pass < 2; ++pass) {
         for (int step = 0; step < tiles; ++step) {
             const int j = pass ? tiles - 1 - step : step;
-            const int i0 = j * tile + at * K;
+            const int i0 = (firstTile + j) * tile + at * K;
             if (tiles > 1) {
                 if (pass == 0) {
                     if (at == 0 && live)
@@ -891,14 +1003,25 @@ __global__ __launch_bounds__(256) void scan_rows_backward_kernel(const ScanParam
                 for (int c = 0; c < G; ++c) h[c] = __shfl(fmaf(A, h[c], U[c]), width - 1, width);
                 continue;
             }
-            joinLanes<G, false>(A2, D, width, lane);
-            const float behind = __shfl_down(A2, 1, width);
-            float kw[G], entry[K][G], dg[K][1];
+            float kw[G], dg[K][1], entry[K][G];
+            if (dp) {
+                joinLanes<G, false>(A2, D, width, lane);
+                const float behind = __shfl_down(A2, 1, width);
 #pragma unroll
-            for (int c = 0; c < G; ++c) {
-                const float d1 = __shfl_down(D[c], 1, width);
-                kw[c] = at + 1 < width ? fmaf(behind, k[c], d1) : k[c];
-                k[c] = __shfl(fmaf(A2, k[c], D[c]), 0, width);
+                for (int c = 0; c < G; ++c) {
+                    const float d1 = __shfl_down(D[c], 1, width);
+                    kw[c] = at + 1 < width ? fmaf(behind, k[c], d1) : k[c];
+                    k[c] = __shfl(fmaf(A2, k[c], D[c]), 0, width);
+                }
+            } else {  // only the last state's gradient comes in: one product of gates for all channels
+                float none[1] = {0.f};
+                joinLanes<1, false>(A2, none, width, lane);
+                const float behind = __shfl_down(A2, 1, width), all = __shfl(A2, 0, width);
+#pragma unroll
+                for (int c = 0; c < G; ++c) {
+                    kw[c] = at + 1 < width ? behind * k[c] : k[c];
+                    k[c] *= all;
+                }
             }
 #pragma unroll
             for (int q = 0; q < K; ++q)
@@ -935,7 +1058,7 @@ __global__ __launch_bounds__(256) void scan_rows_backward_kernel(const ScanParam
             }
         }
     }
-    if (p.dh0 && live && at == 0)
+    if (p.dh0 && live && at == 0 && span == 0)
 #pragma unroll
         for (int c = 0; c < G; ++c) p.dh0[state + c] = k[c];
 }
@@ -1000,12 +1123,18 @@ ScanPlan planScan(const ScanParams& p, int dtype, bool backward) {
     // gates beside each other to fill half a wave.
     plan.rows = p.G <= 4 && (p.Cg < 32 || step < next);
     if (plan.rows) {
-        const int K = backward ? kRowStepsBackward : kRowSteps;
-        plan.width = std::min(64, powerOfTwoAtLeast((p.T + K - 1) / std::max(K, 1)));
-        plan.tile = plan.width * K;
-        const long long tiles = (p.T + (long long)plan.tile - 1) / plan.tile;
-        plan.chunkSteps = p.T;
-        plan.wsFloats = backward && tiles > 1 ? size_t(p.B) * p.C * tiles : 0;
+        plan.width = std::min(64, powerOfTwoAtLeast((p.T + kRowSteps - 1) / kRowSteps));
+        plan.tile = plan.width * kRowSteps;
+        const int tiles = std::max(1, int((p.T + (long long)plan.tile - 1) / plan.tile));
+        // Spans while there are fewer than 8 waves of rows for each CU (a row of several tiles is a wave)
+        const long long rows = p.B * p.Cg, want = tiles > 1 ? (2048 + rows - 1) / rows : 1;
+        const int tilesOfSpan = int((tiles + std::min(want, (long long)tiles) - 1) / std::min(want, (long long)tiles));
+        plan.chunks = (tiles + tilesOfSpan - 1) / tilesOfSpan;
+        plan.chunkSteps = tilesOfSpan * plan.tile;
+        ScanParams q = p;
+        q.ws = nullptr;
+        plan.wsFloats = plan.chunks > 1 ? size_t(rowScratch(q, plan, backward).heads - q.ws) : 0;
+        if (backward && tilesOfSpan > 1) plan.wsFloats += size_t(rows) * plan.chunks * tilesOfSpan * p.G;
         return plan;
     }
     // Channels of a lane.  A gate's two to four, if they are adjacent: its factor is worked out once and its gradient summed in the lane.  Otherwise
@@ -1044,9 +1173,14 @@ hipError_t launch_gated_scan(const ScanParams& p, const ScanPlan& plan, int dtyp
     return withType(dtype, [&](auto element) {
         typedef decltype(element) T;
         if (plan.rows) {
-            const unsigned grid = unsigned((p.B * p.Cg * plan.width + 255) / 256);
+            const dim3 grid(unsigned((p.B * p.Cg * plan.width + 255) / 256), unsigned(plan.chunks));
+            const bool beside = gateBeside(p.x, p.xs, p.gate, p.gs, p, sizeof(T));
             return withGroup(p.G, [&](auto g) {
-                scan_rows_kernel<T, decltype(g)::value><<<grid, 256, 0, s>>>(p, plan.width, gateBeside(p.x, p.xs, p.gate, p.gs, p, sizeof(T)));
+                if (plan.chunks > 1) {
+                    scan_rows_spans_kernel<T, decltype(g)::value, false><<<grid, 256, 0, s>>>(p, plan, beside);
+                    if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+                }
+                scan_rows_kernel<T, decltype(g)::value><<<grid, 256, 0, s>>>(p, plan, beside);
                 return hipGetLastError();
             });
         }
@@ -1074,10 +1208,15 @@ hipError_t launch_gated_scan_backward(const ScanParams& p, const ScanPlan& plan,
     return withType(dtype, [&](auto element) {
         typedef decltype(element) T;
         if (plan.rows) {
-            const unsigned grid = unsigned((p.B * p.Cg * plan.width + 255) / 256);
+            const dim3 grid(unsigned((p.B * p.Cg * plan.width + 255) / 256), unsigned(plan.chunks));
+            const bool beside = gateBeside(p.x, p.xs, p.gate, p.gs, p, sizeof(T));
+            const bool outBeside = p.dx && p.dgate && gateBeside(p.dx, p.dxs, p.dgate, p.dgs, p, sizeof(T));
             return withGroup(p.G, [&](auto g) {
-                scan_rows_backward_kernel<T, decltype(g)::value><<<grid, 256, 0, s>>>(
-                    p, plan.width, gateBeside(p.x, p.xs, p.gate, p.gs, p, sizeof(T)), p.dx && p.dgate && gateBeside(p.dx, p.dxs, p.dgate, p.dgs, p, sizeof(T)));
+                if (plan.chunks > 1) {
+                    scan_rows_spans_kernel<T, decltype(g)::value, true><<<grid, 256, 0, s>>>(p, plan, beside);
+                    if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+                }
+                scan_rows_backward_kernel<T, decltype(g)::value><<<grid, 256, 0, s>>>(p, plan, beside, outBeside);
                 return hipGetLastError();
             });
         }

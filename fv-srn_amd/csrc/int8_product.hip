@@ -17,80 +17,82 @@ typedef int int16_t_ __attribute__((ext_vector_type(16)));
 // codes and scales
 // ---------------------------------------------------------------------------------------------------------------------
 
-// Bound by memory: every value is read once and a quarter or half of its bytes written.  `width` lanes share a row, 8 values of each in turn
-// (rows longer than 8 width HELD are read a second time, from the caches).
-constexpr int kHeld = 8;
-
-template <class T, bool ALIGNED>
-__device__ __forceinline__ void loadEight(const T* row, int k, int cols, float (&v)[8]) {
-    if (ALIGNED && k + 8 <= cols) {
-        const Pack<T, 8> x = *reinterpret_cast<const Pack<T, 8>*>(row + k);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = toFloat(x.v[j]);
+// Bound by memory: every value is read once and a quarter or half of its bytes written.  `width` lanes share a row, 8 values of each in turn, in registers
+// from the maximum to the codes (of rows longer than 8 width HELD the rest is read a second time, from the caches).  Short rows go ROWS at a time: one
+// 16-byte load a lane would leave the memory idle.  Any alignment: the loads and stores of 8 values are as fast as the lines they touch.
+template <class T>
+__device__ __forceinline__ void loadEight(const T* row, int k, int cols, T (&v)[8]) {
+    if (k + 8 <= cols) {
+        loadWide<T, 8>(v, row + k);
     } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = k + j < cols ? toFloat(row[k + j]) : 0.f;
+        for (int j = 0; j < 8; ++j) v[j] = k + j < cols ? row[k + j] : T(0.f);
     }
 }
 
-template <bool ALIGNED>
-__device__ __forceinline__ void storeEight(signed char* row, int k, int cols, const float (&v)[8], float scale, bool zero) {
-    Pack<signed char, 8> q;
+template <class T>
+__device__ __forceinline__ void storeEight(signed char* row, int k, int cols, const T (&v)[8], float scale, bool zero) {
+    signed char q[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) q.v[j] = zero ? 0 : (signed char)int(__builtin_rintf(__fdiv_rn(v[j], scale)));  // (the definition's quotient: rounded to 32 bits)
-    if (ALIGNED && k + 8 <= cols) {
-        *reinterpret_cast<Pack<signed char, 8>*>(row + k) = q;
+    for (int j = 0; j < 8; ++j) q[j] = zero ? 0 : (signed char)int(__builtin_rintf(__fdiv_rn(toFloat(v[j]), scale)));  // (the definition's quotient: rounded to 32 bits)
+    if (k + 8 <= cols) {
+        storeWide<signed char, 8>(row + k, q);
     } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-            if (k + j < cols) row[k + j] = q.v[j];
+            if (k + j < cols) row[k + j] = q[j];
     }
 }
 
-// ALIGNED: row starts are multiples of 8 elements in x and of 8 bytes in the codes
-template <class T, bool ALIGNED, int HELD>
+template <class T, int HELD, int ROWS>
 __global__ __launch_bounds__(256) void quantize_rows_kernel(const QuantizeParams p, const int width) {
-    const int lane = threadIdx.x & 63, at = lane & (width - 1);
-    const long long own = (blockIdx.x * 4LL + (threadIdx.x >> 6)) * (64 / width) + lane / width, row = min(own, p.rows - 1);
-    const T* const x = static_cast<const T*>(p.x) + row * p.ldx;
-    float v[HELD][8], most = 0.f, odd = 0.f;
+    const int lane = threadIdx.x & 63, at = lane & (width - 1), group = (threadIdx.x >> 6) * (64 / width) + lane / width, groups = 4 * (64 / width);
+    const long long first = blockIdx.x * (long long)(groups * ROWS) + group;  // rows first, first + groups, ...
+    T v[ROWS][HELD][8];
 #pragma unroll
-    for (int j = 0; j < HELD; ++j) {
-        const int k = (j * width + at) * 8;
-        loadEight<T, ALIGNED>(x, min(k, p.cols), p.cols, v[j]);
+    for (int r = 0; r < ROWS; ++r) {
+        const T* const x = static_cast<const T*>(p.x) + min(first + r * groups, p.rows - 1) * p.ldx;
+#pragma unroll
+        for (int j = 0; j < HELD; ++j) loadEight(x, (j * width + at) * 8, p.cols, v[r][j]);
     }
-    auto look = [&](const float(&w)[8]) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            most = fmaxf(most, fabsf(w[e]));
-            odd += w[e] * 0.f;  // (NaN once a value is no finite number)
+    for (int r = 0; r < ROWS; ++r) {
+        const long long row = min(first + r * groups, p.rows - 1);
+        const T* const x = static_cast<const T*>(p.x) + row * p.ldx;
+        float most = 0.f, odd = 0.f;
+        auto look = [&](const T(&w)[8]) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                most = fmaxf(most, fabsf(toFloat(w[e])));
+                odd = fmaf(toFloat(w[e]), 0.f, odd);  // (NaN once a value is no finite number)
+            }
+        };
+#pragma unroll
+        for (int j = 0; j < HELD; ++j) look(v[r][j]);
+        for (int k = (HELD * width + at) * 8; k < p.cols; k += width * 8) {
+            T w[8];
+            loadEight(x, k, p.cols, w);
+            look(w);
         }
-    };
+        for (int o = 1; o < width; o <<= 1) {
+            most = fmaxf(most, __shfl_xor(most, o, 64));
+            odd += __shfl_xor(odd, o, 64);
+        }
+        if (first + r * groups >= p.rows) return;
+        const bool bad = odd != odd;
+        const float scale = fmaxf(most * (1.f / 127.f), 0x1p-126f);
+        if (at == 0) p.scales[row] = bad ? __builtin_nanf("") : scale;
+        signed char* const q = p.codes + row * p.ldc;
 #pragma unroll
-    for (int j = 0; j < HELD; ++j) look(v[j]);
-    for (int k = (HELD * width + at) * 8; k < p.cols; k += width * 8) {
-        float w[8];
-        loadEight<T, ALIGNED>(x, k, p.cols, w);
-        look(w);
-    }
-    for (int o = 1; o < width; o <<= 1) {
-        most = fmaxf(most, __shfl_xor(most, o, 64));
-        odd += __shfl_xor(odd, o, 64);
-    }
-    if (own >= p.rows) return;
-    const bool bad = odd != odd;
-    const float scale = fmaxf(most * (1.f / 127.f), 0x1p-126f);
-    if (at == 0) p.scales[row] = bad ? __builtin_nanf("") : scale;
-    signed char* const q = p.codes + row * p.ldc;
-#pragma unroll
-    for (int j = 0; j < HELD; ++j) {
-        const int k = (j * width + at) * 8;
-        if (k < p.cols) storeEight<ALIGNED>(q, k, p.cols, v[j], scale, bad);
-    }
-    for (int k = (HELD * width + at) * 8; k < p.cols; k += width * 8) {
-        float w[8];
-        loadEight<T, ALIGNED>(x, k, p.cols, w);
-        storeEight<ALIGNED>(q, k, p.cols, w, scale, bad);
+        for (int j = 0; j < HELD; ++j) {
+            const int k = (j * width + at) * 8;
+            if (k < p.cols) storeEight(q, k, p.cols, v[r][j], scale, bad);
+        }
+        for (int k = (HELD * width + at) * 8; k < p.cols; k += width * 8) {
+            T w[8];
+            loadEight(x, k, p.cols, w);
+            storeEight(q, k, p.cols, w, scale, bad);
+        }
     }
 }
 
@@ -420,18 +422,18 @@ hipError_t withType(int dtype, F&& f) {
 hipError_t launch_quantize_rows(const QuantizeParams& p, int dtype, hipStream_t s) {
     return withType(dtype, [&](auto element) {
         typedef decltype(element) T;
-        const bool aligned = multipleOf(p.x, 8 * sizeof(T)) && p.ldx % 8 == 0 && multipleOf(p.codes, 8) && p.ldc % 8 == 0;
         const int width = std::min(64, powerOfTwoAtLeast((p.cols + 7) / 8));
-        const unsigned grid = unsigned((p.rows + 4 * (64 / width) - 1) / (4 * (64 / width)));
-        auto launch = [&](auto held) {
-            constexpr int H = decltype(held)::value;
-            if (aligned) quantize_rows_kernel<T, true, H><<<grid, 256, 0, s>>>(p, width);
-            else quantize_rows_kernel<T, false, H><<<grid, 256, 0, s>>>(p, width);
+        auto launch = [&](auto held, auto rows) {
+            constexpr int H = decltype(held)::value, R = decltype(rows)::value;
+            const long long rowsOfBlock = 4 * (64 / width) * R;
+            quantize_rows_kernel<T, H, R><<<unsigned((p.rows + rowsOfBlock - 1) / rowsOfBlock), 256, 0, s>>>(p, width);
             return hipGetLastError();
         };
-        if (p.cols <= 512) return launch(std::integral_constant<int, 1>{});
-        if (p.cols <= 2048) return launch(std::integral_constant<int, 4>{});
-        return launch(std::integral_constant<int, kHeld>{});
+        // (rows at a time: only where there are enough of them for 8 waves on each CU all the same)
+        if (p.cols <= 512 && p.rows * width >= 4LL * 64 * 2048) return launch(std::integral_constant<int, 1>{}, std::integral_constant<int, 4>{});
+        if (p.cols <= 512) return launch(std::integral_constant<int, 1>{}, std::integral_constant<int, 1>{});
+        if (p.cols <= 2048) return launch(std::integral_constant<int, 4>{}, std::integral_constant<int, 1>{});
+        return launch(std::integral_constant<int, 8>{}, std::integral_constant<int, 1>{});
     });
 }
 

@@ -27,6 +27,7 @@ FVSRN_PIECE(16, 2, uint4_piece)
 FVSRN_PIECE(8, 2, uint2_piece)
 FVSRN_PIECE(4, 2, unsigned)
 FVSRN_PIECE(2, 2, unsigned short)
+FVSRN_PIECE(8, 1, uint2_piece)
 #undef FVSRN_PIECE
 
 constexpr int pieceOf(int bytes) { return bytes >= 16 ? 16 : bytes >= 8 ? 8 : bytes >= 4 ? 4 : 2; }

@@ -137,7 +137,8 @@ def modes(i):
 # tiles shared by waves, cut into spans; gates of 2, 8, 100 and 130 channels
 SHAPES = [(1, 1, 1, 1), (3, 1, 12, 4), (1, 1, 300, 100), (2, 2, 5, 5), (5, 37, 3, 1), (2, 512, 3, 1), (3, 513, 4, 1), (2, 2049, 2, 1), (300, 9, 1, 1), (1, 1000, 4, 2),
           (2, 16, 64, 64), (2, 33, 40, 40), (2, 130, 65, 65), (1, 300, 100, 100), (1, 3000, 70, 70), (2, 1500, 96, 12), (3, 257, 200, 2), (1, 600, 130, 1), (2, 100, 66, 33),
-          (1, 5000, 1, 1), (1, 20, 270000, 270000), (1, 40, 90000, 30000), (1, 129, 5, 1)]
+          (1, 5000, 1, 1), (1, 20, 270000, 270000), (1, 40, 90000, 30000), (1, 129, 5, 1), (300, 4500, 1, 1),
+          (3, 9000, 4, 4), (1, 20000, 2, 1), (1, 700, 128, 128), (2, 700, 512, 512), (1, 300, 300, 150)]
 
 
 @pytest.mark.gpu
@@ -376,7 +377,7 @@ def assert_codes(x, codes, scales):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=["f32", "f16", "bf16"])
-@pytest.mark.parametrize("rows,cols", [(1, 1), (5, 7), (3, 8), (700, 9), (33, 63), (2, 64), (129, 250), (64, 256), (3, 511), (7, 513), (9, 2049), (5, 4096), (2, 5003), (1, 20000)])
+@pytest.mark.parametrize("rows,cols", [(1, 1), (5, 7), (3, 8), (700, 9), (33, 63), (2, 64), (129, 250), (64, 256), (3, 511), (7, 513), (9, 2049), (5, 4096), (2, 5003), (1, 20000), (20003, 250), (70001, 40)])
 def test_codes_and_scales(rows, cols, dtype):
     x = (torch.randn(rows, cols, generator=torch.Generator().manual_seed(rows * cols)) * 3).to(dtype).cuda()
     assert_codes(x, *capi.quantize_rows(x))
