@@ -612,7 +612,10 @@ __global__ __launch_bounds__(256) void scan_gate_sum_kernel(const ScanParams p, 
 // lanes are steps
 // ---------------------------------------------------------------------------------------------------------------------
 
-constexpr int kRowSteps = 8;  // steps of a lane
+// Steps of a lane: 8, and backward 4 for rows of up to 256 steps, which are one tile either way (65536 rays x 256 with gradients: 102 us with 4 steps, whose
+// registers leave room for more waves, against 130 with 8; 262144 x 512, two tiles against one: 1018 against 899).
+constexpr int kRowSteps = 8, kRowStepsShort = 4;
+constexpr int rowSteps(int T, bool backward) { return backward && T <= 64 * kRowStepsShort ? kRowStepsShort : kRowSteps; }
 
 // (A, U) of this lane's span joined with its row's lanes before it (FORWARD) or behind it, over the `width` lanes of a row: an inclusive scan.
 template <int G, bool FORWARD>
@@ -916,9 +919,8 @@ __global__ __launch_bounds__(256) void scan_rows_kernel(const ScanParams p, cons
         for (int c = 0; c < G; ++c) p.last[state + c] = h[c];
 }
 
-template <class T, int G>
+template <class T, int G, int K>
 __global__ __launch_bounds__(256) void scan_rows_backward_kernel(const ScanParams p, const ScanPlan plan, const bool beside, const bool outBeside) {
-    constexpr int K = kRowSteps;
     const int width = plan.width, lane = threadIdx.x & 63, at = lane & (width - 1), span = blockIdx.y;
     const long long rows = p.B * p.Cg, own = (blockIdx.x * 4LL + (threadIdx.x >> 6)) * (64 / width) + lane / width;
     const bool live = own < rows;
@@ -1123,8 +1125,9 @@ ScanPlan planScan(const ScanParams& p, int dtype, bool backward) {
     // gates beside each other to fill half a wave.
     plan.rows = p.G <= 4 && (p.Cg < 32 || step < next);
     if (plan.rows) {
-        plan.width = std::min(64, powerOfTwoAtLeast((p.T + kRowSteps - 1) / kRowSteps));
-        plan.tile = plan.width * kRowSteps;
+        const int K = rowSteps(p.T, backward);
+        plan.width = std::min(64, powerOfTwoAtLeast((p.T + K - 1) / K));
+        plan.tile = plan.width * K;
         const int tiles = std::max(1, int((p.T + (long long)plan.tile - 1) / plan.tile));
         // Spans while there are fewer than 8 waves of rows for each CU (a row of several tiles is a wave)
         const long long rows = p.B * p.Cg, want = tiles > 1 ? (2048 + rows - 1) / rows : 1;
@@ -1216,7 +1219,8 @@ hipError_t launch_gated_scan_backward(const ScanParams& p, const ScanPlan& plan,
                     scan_rows_spans_kernel<T, decltype(g)::value, true><<<grid, 256, 0, s>>>(p, plan, beside);
                     if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
                 }
-                scan_rows_backward_kernel<T, decltype(g)::value><<<grid, 256, 0, s>>>(p, plan, beside, outBeside);
+                if (rowSteps(p.T, true) == kRowStepsShort) scan_rows_backward_kernel<T, decltype(g)::value, kRowStepsShort><<<grid, 256, 0, s>>>(p, plan, beside, outBeside);
+                else scan_rows_backward_kernel<T, decltype(g)::value, kRowSteps><<<grid, 256, 0, s>>>(p, plan, beside, outBeside);
                 return hipGetLastError();
             });
         }

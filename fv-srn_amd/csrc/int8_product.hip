@@ -30,17 +30,30 @@ __device__ __forceinline__ void loadEight(const T* row, int k, int cols, T (&v)[
     }
 }
 
+// The codes are the quotients v / scale rounded to 32 bits, rounded to integers.  A division is ten instructions, and they would be what the kernel waits for: where it
+// can be, the quotient is q = v y with y = 1 / scale rounded, corrected by its exact remainder, q + (v - q scale) y, which is the rounded quotient
+// (Markstein's theorem: y correctly rounded, the divisor's significand not all ones, nothing subnormal: `exact` says so).  Adding 1.5 2^23 leaves the nearest integer
+// (ties to even) in the low bits.
 template <class T>
-__device__ __forceinline__ void storeEight(signed char* row, int k, int cols, const T (&v)[8], float scale, bool zero) {
-    signed char q[8];
+__device__ __forceinline__ void storeEight(signed char* row, int k, int cols, const T (&v)[8], float scale, float y, bool exact, bool zero) {
+    unsigned w[8], word[2];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) q[j] = zero ? 0 : (signed char)int(__builtin_rintf(__fdiv_rn(toFloat(v[j]), scale)));  // (the definition's quotient: rounded to 32 bits)
+    for (int j = 0; j < 8; ++j) {
+        const float x = toFloat(v[j]), q = x * y;
+        const float quotient = exact ? fmaf(fmaf(-q, scale, x), y, q) : __fdiv_rn(x, scale);
+        w[j] = __float_as_uint(quotient + 12582912.f);
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {  // the low bytes of four words
+        const unsigned lo = __builtin_amdgcn_perm(w[4 * j + 1], w[4 * j], 0x0c0c0400u), hi = __builtin_amdgcn_perm(w[4 * j + 3], w[4 * j + 2], 0x04000c0cu);
+        word[j] = zero ? 0u : lo | hi;
+    }
     if (k + 8 <= cols) {
-        storeWide<signed char, 8>(row + k, q);
+        storeWide<signed char, 8>(row + k, reinterpret_cast<const signed char*>(word));
     } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-            if (k + j < cols) row[k + j] = q[j];
+            if (k + j < cols) row[k + j] = (signed char)(word[j >> 2] >> (8 * (j & 3)));
     }
 }
 
@@ -80,18 +93,25 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const QuantizeParams
         }
         if (first + r * groups >= p.rows) return;
         const bool bad = odd != odd;
+        signed char* const q = p.codes + row * p.ldc;
         const float scale = fmaxf(most * (1.f / 127.f), 0x1p-126f);
         if (at == 0) p.scales[row] = bad ? __builtin_nanf("") : scale;
-        signed char* const q = p.codes + row * p.ldc;
+        const float y = __fdiv_rn(1.f, scale);
+        const bool exact = scale > 0x1p-90f && (__float_as_uint(scale) & 0x7fffffu) != 0x7fffffu;
+        auto store = [&](const T(&w)[8], int k) {
+            // (a branch per row and not a choice per value)
+            if (exact) storeEight(q, k, p.cols, w, scale, y, true, bad);
+            else storeEight(q, k, p.cols, w, scale, y, false, bad);
+        };
 #pragma unroll
         for (int j = 0; j < HELD; ++j) {
             const int k = (j * width + at) * 8;
-            if (k < p.cols) storeEight(q, k, p.cols, v[r][j], scale, bad);
+            if (k < p.cols) store(v[r][j], k);
         }
         for (int k = (HELD * width + at) * 8; k < p.cols; k += width * 8) {
             T w[8];
             loadEight(x, k, p.cols, w);
-            storeEight(q, k, p.cols, w, scale, bad);
+            store(w, k);
         }
     }
 }
@@ -266,18 +286,19 @@ __global__ __launch_bounds__(256) void matmul_int8_kernel(const Int8Params p, co
 }
 
 // Aligned rows: a tile of TM tokens x TN channels for WM x WN waves, each with PM x 2 pieces of 32 x 32, 64 bytes of k a stage.
-//   Stages go from memory into LDS without passing a register, into a ring of four: while one is multiplied three travel (a stage of 256 x 256 is multiplied in
+//   Stages go from memory into LDS without passing a register, into a ring of RING: while one is multiplied the others travel (a stage of 256 x 256 is multiplied in
 // 0.4 us, which is less than the way from memory).  The wait for the next stage and the barrier stand between the two halves of a stage's products, and the
 // operands of a half are read while the half before is multiplied, so the matrix units have work queued at every wait.
 //   LDS holds rows of four 16-byte chunks, chunk c of row r at place c ^ swizzle(r), so that the 32 rows a wave reads at one k spread over all banks; the
 // loads write LDS in lane order, so it is their source that is permuted.  A wave's channels are paired -- column l of its piece j is channel 2 l + j -- so that a
 // lane stores two adjacent outputs and a wave whole 128-byte lines of 16-bit ones.
-template <class T, int TM, int TN, int WM, int WN>
+template <class T, int TM, int TN, int WM, int WN, int RING>
 __global__ __launch_bounds__(64 * WM * WN) void matmul_int8_tile_kernel(const Int8Params p, const int activation, const int tilesM, const int tilesN) {
-    constexpr int BK = 64, RING = 4, WAVES = WM * WN, PM = TM / WM / 32, STAGE = (TM + TN) * BK;
+    constexpr int BK = 64, WAVES = WM * WN, PM = TM / WM / 32, STAGE = (TM + TN) * BK;
     static_assert(TN / WN == 64, "a wave's channels are paired");
     constexpr int LOADS = STAGE / 1024 / WAVES;  // of a wave, 1 KiB each: 16 rows
-    static_assert(LOADS == 4, "the waits below count loads");
+    static_assert(STAGE % (1024 * WAVES) == 0 && LOADS * (RING - 2) < 64, "the waits below count loads");
+    constexpr int FLOWING = LOADS * (RING - 2);  // loads that may still be on their way when the next stage is waited for
     __shared__ __attribute__((aligned(1024))) signed char lds[RING][STAGE];
     __shared__ __attribute__((aligned(16))) float scaleA[TM], scaleB[TN], bias[TN];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -336,11 +357,11 @@ __global__ __launch_bounds__(64 * WM * WN) void matmul_int8_tile_kernel(const In
         scaleB[e] = p.scaleB[n];
         bias[e] = p.bias ? p.bias[n] : 0.f;
     }
-    // The next stage is everybody's to read behind the barrier, and nobody reads the one before it any more.  Two stages may still be on their way (8
+    // The next stage is everybody's to read behind the barrier, and nobody reads the one before it any more.  RING - 2 stages may still be on their way (FLOWING
     // loads of this wave); at the end of k all have to be there.
     auto arrive = [&](bool flowing) {
-        if (flowing) __builtin_amdgcn_s_waitcnt(0x0078);  // vmcnt(8) lgkmcnt(0)
-        else __builtin_amdgcn_s_waitcnt(0x0070);          // vmcnt(0) lgkmcnt(0)
+        if (flowing) __builtin_amdgcn_s_waitcnt((FLOWING & 15) | (FLOWING >> 4) << 14 | 0x0070);  // vmcnt(FLOWING) lgkmcnt(0)
+        else __builtin_amdgcn_s_waitcnt(0x0070);                                                  // vmcnt(0) lgkmcnt(0)
         asm volatile("s_barrier" ::: "memory");
     };
     for (int s = 0; s < min(RING - 1, stages); ++s) load(s);
@@ -455,12 +476,16 @@ hipError_t launch_matmul_int8(const Int8Params& p, int activation, int outDtype,
         if (p.M <= 64) return aligned ? fewOf(std::true_type{}) : fewOf(std::false_type{});
         auto tiles = [&](int edge) { return ((p.M + edge - 1) / edge) * ((p.N + edge - 1) / edge); };
         if (aligned && p.N > 32 && tiles(64) < (1LL << 24)) {
-            if (tiles(256) >= 256 && p.K >= 1024)
-                matmul_int8_tile_kernel<T, 256, 256, 2, 4><<<unsigned(tiles(256)), 512, 0, s>>>(p, activation, int((p.M + 255) / 256), (p.N + 255) / 256);
-            else if (tiles(128) >= 256)
-                matmul_int8_tile_kernel<T, 128, 128, 2, 2><<<unsigned(tiles(128)), 256, 0, s>>>(p, activation, int((p.M + 127) / 128), (p.N + 127) / 128);
-            else
-                matmul_int8_tile_kernel<T, 64, 64, 2, 1><<<unsigned(tiles(64)), 128, 0, s>>>(p, activation, int((p.M + 63) / 64), (p.N + 63) / 64);
+            // The largest tile that still gives every CU one (edges of 256 only with k long enough to hide their beginning and end: one fits a CU). 8192 x
+            // 4096 x 4096: 145 us with 256, 199 with 128, 300 with 64; 262144 x 256 x 256: 46, 43, 61 us; 2048 x 1024 x 1024: 16, 10, 9 us.
+            auto launch = [&](auto edge, auto wavesM, auto wavesN, auto ring) {
+                constexpr int E = decltype(edge)::value, WM = decltype(wavesM)::value, WN = decltype(wavesN)::value;
+                matmul_int8_tile_kernel<T, E, E, WM, WN, decltype(ring)::value><<<unsigned(tiles(E)), 64 * WM * WN, 0, s>>>(p, activation, int((p.M + E - 1) / E), (p.N + E - 1) / E);
+            };
+            using std::integral_constant;
+            if (tiles(256) >= 256 && p.K >= 1024) launch(integral_constant<int, 256>{}, integral_constant<int, 4>{}, integral_constant<int, 4>{}, integral_constant<int, 3>{});
+            else if (tiles(128) >= 256) launch(integral_constant<int, 128>{}, integral_constant<int, 2>{}, integral_constant<int, 2>{}, integral_constant<int, 3>{});
+            else launch(integral_constant<int, 64>{}, integral_constant<int, 2>{}, integral_constant<int, 1>{}, integral_constant<int, 4>{});
             return hipGetLastError();
         }
         const dim3 grid(unsigned((p.M + 63) / 64), unsigned((p.N + 63) / 64));
