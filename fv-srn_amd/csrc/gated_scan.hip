@@ -57,8 +57,10 @@ __device__ __forceinline__ int positionOf(int i, int n, int reverse) { return re
 
 constexpr int kScanWaves = 8;  // waves that share a tile
 // steps of a wave that are held in registers, for V channels of a lane
-constexpr int forwardSteps(int V) { return V <= 2 ? 16 : 8; }
-constexpr int backwardSteps(int V) { return V <= 2 ? 8 : 4; }
+// (twice as many cost more waves than they hide latency: series of 65536 x 1024 bf16 150 us against 132; backward, 16-bit pairs are better off with 8 steps and
+// the four registers they spill at four waves a SIMD: 224 us against 259)
+constexpr int forwardSteps(int V) { return V == 1 ? 16 : V == 2 ? 8 : 4; }
+constexpr int backwardSteps(int V, int elementBytes) { return V == 1 || (V == 2 && elementBytes == 2) ? 8 : 4; }
 
 // What a lane stands for: V adjacent channels, each with a gate of its own, or (SHARED) the V channels of one gate.  V == 1 and slots > 1 (backward, gates
 // of many channels): `slots` lanes of a gate's channels -- padded to a power of two, so that their sum is a butterfly of shuffles -- and, for
@@ -115,28 +117,28 @@ __device__ __forceinline__ void loadChannels(const T* p, long long step, int i, 
     }
 }
 
-// The gates of steps i .. i + L - 1 (1 from step `end` on); rest: the factor of x, 1 - a of BLEND and 1 of ADD
-template <class T, int V, int L>
-__device__ __forceinline__ void gatesOf(const ScanParams& p, const T (&raw)[L][V], int i, int end, float (&a)[L][V], float (&rest)[L][V]) {
+// The gates of steps i .. i + L - 1 (1 from step `end` on), and the factor of x: 1 - a of BLEND, 1 of ADD.  use(k, v, a, factor)
+template <class T, int V, int L, class F>
+__device__ __forceinline__ void withGates(const ScanParams& p, const T (&raw)[L][V], int i, int end, F&& use) {
     if (p.exp) {
 #pragma unroll
         for (int k = 0; k < L; ++k)
 #pragma unroll
-            for (int v = 0; v < V; ++v) gateOf<true>(toFloat(raw[k][v]), p.scale, a[k][v], rest[k][v]);
+            for (int v = 0; v < V; ++v) {
+                float a, rest;
+                gateOf<true>(toFloat(raw[k][v]), p.scale, a, rest);
+                use(k, v, a, p.blend ? rest : 1.f);
+            }
     } else {
 #pragma unroll
         for (int k = 0; k < L; ++k)
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                gateOf<false>(toFloat(raw[k][v]), p.scale, a[k][v], rest[k][v]);
-                if (i + L > end && i + k >= end) a[k][v] = 1.f;  // (read as 0; a gate of 0 in EXP is 1 already, and x is 0)
+                float a, rest;
+                gateOf<false>(toFloat(raw[k][v]), p.scale, a, rest);
+                if (i + L > end && i + k >= end) a = 1.f;  // (read as 0; a gate of 0 in EXP is 1 already, and x is 0)
+                use(k, v, a, p.blend ? rest : 1.f);
             }
-    }
-    if (!p.blend) {
-#pragma unroll
-        for (int k = 0; k < L; ++k)
-#pragma unroll
-            for (int v = 0; v < V; ++v) rest[k][v] = 1.f;
     }
 }
 
@@ -194,23 +196,20 @@ __global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW) void scan_channels_kernel(
         T rawG[L][GV], rawX[L][V];
         loadChannels<T, GV, L>(gp, p.gs[1], i0, n, inside, p.reverse, rawG);
         loadChannels<T, V, L>(xp, p.xs[1], i0, n, inside, p.reverse, rawX);
-        float a[L][GV], rest[L][GV], u[L][V], a2[GV], u2[V];
-        gatesOf<T, GV, L>(p, rawG, i0, inside, a, rest);
+        float a[L][GV], u[L][V], a2[GV], u2[V];
 #pragma unroll
         for (int v = 0; v < V; ++v) u2[v] = 0.f;
 #pragma unroll
         for (int v = 0; v < GV; ++v) a2[v] = 1.f;
+        withGates<T, GV, L>(p, rawG, i0, inside, [&](int k, int v, float gate, float factor) {
+            a[k][v] = gate;
+            a2[v] *= gate;
 #pragma unroll
-        for (int k = 0; k < L; ++k) {
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                u[k][v] = rest[k][SHARED ? 0 : v] * toFloat(rawX[k][v]);
-                if (NW > 1 || AGGREGATE) u2[v] = fmaf(a[k][SHARED ? 0 : v], u2[v], u[k][v]);
+            for (int c = SHARED ? 0 : v; c < (SHARED ? V : v + 1); ++c) {
+                u[k][c] = factor * toFloat(rawX[k][c]);
+                u2[c] = fmaf(gate, u2[c], u[k][c]);
             }
-            if (NW > 1 || AGGREGATE)
-#pragma unroll
-                for (int v = 0; v < GV; ++v) a2[v] *= a[k][v];
-        }
+        });
         float pre[V];
 #pragma unroll
         for (int v = 0; v < V; ++v) pre[v] = h[v];
@@ -220,7 +219,7 @@ __global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW) void scan_channels_kernel(
 #pragma unroll
             for (int v = 0; v < V; ++v) joined[buffer][w][GV + v][lane] = u2[v];
             __syncthreads();  // (one barrier a tile: the two buffers take turns, and a wave can only be one tile ahead)
-#pragma unroll
+#pragma unroll 2
             for (int j = 0; j < NW; ++j) {
                 float aj[GV];
 #pragma unroll
@@ -299,7 +298,7 @@ inline size_t backwardFloats(const ScanParams& p, const ScanPlan& plan) {
 // Backward, first launch of a call that is cut into spans
 template <class T, int NW, int V, bool SHARED>
 __global__ __launch_bounds__(64 * NW) void scan_channels_spans_kernel(const ScanParams p, const ScanPlan plan, const int blocks) {
-    constexpr int L = backwardSteps(V), GV = SHARED ? 1 : V;
+    constexpr int L = backwardSteps(V, sizeof(T)), GV = SHARED ? 1 : V;
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     const long long b = blockIdx.x / blocks;
     const ChannelLane ch = channelLane<V, SHARED>(p, int(blockIdx.x % blocks), lane, plan.slots, plan.parts);
@@ -333,22 +332,19 @@ __global__ __launch_bounds__(64 * NW) void scan_channels_spans_kernel(const Scan
         loadChannels<T, GV, L>(gp, p.gs[1], i0, n, end, p.reverse, rawG);
         loadChannels<T, V, L>(xp, p.xs[1], i0, n, end, p.reverse, rawX);
         if (dp) loadChannels<T, V, L>(dp, p.ds[1], i0, n, end, p.reverse, rawD);
-        float a[L][GV], rest[L][GV], a2[GV], u2[V], d2[V];
-        gatesOf<T, GV, L>(p, rawG, i0, end, a, rest);
+        float a2[GV], u2[V], d2[V];
 #pragma unroll
         for (int v = 0; v < V; ++v) u2[v] = d2[v] = 0.f;
 #pragma unroll
         for (int v = 0; v < GV; ++v) a2[v] = 1.f;
+        withGates<T, GV, L>(p, rawG, i0, end, [&](int k, int v, float gate, float factor) {
+            a2[v] *= gate;
 #pragma unroll
-        for (int k = 0; k < L; ++k) {
-#pragma unroll
-            for (int v = 0; v < GV; ++v) a2[v] *= a[k][v];
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                u2[v] = fmaf(a[k][SHARED ? 0 : v], u2[v], rest[k][SHARED ? 0 : v] * toFloat(rawX[k][v]));
-                if (dp) d2[v] = fmaf(a2[SHARED ? 0 : v], toFloat(rawD[k][v]), d2[v]);
+            for (int c = SHARED ? 0 : v; c < (SHARED ? V : v + 1); ++c) {
+                u2[c] = fmaf(gate, u2[c], factor * toFloat(rawX[k][c]));
+                if (dp) d2[c] = fmaf(a2[v], toFloat(rawD[k][c]), d2[c]);
             }
-        }
+        });
 #pragma unroll
         for (int v = 0; v < GV; ++v) joined[buffer][w][v][lane] = a2[v];
 #pragma unroll
@@ -357,7 +353,7 @@ __global__ __launch_bounds__(64 * NW) void scan_channels_spans_kernel(const Scan
             joined[buffer][w][GV + V + v][lane] = d2[v];
         }
         __syncthreads();
-#pragma unroll
+#pragma unroll 2
         for (int s = 0; s < NW; ++s) {
             float as[GV];
 #pragma unroll
@@ -383,8 +379,8 @@ __global__ __launch_bounds__(64 * NW) void scan_channels_spans_kernel(const Scan
 }
 
 template <class T, int NW, int V, bool SHARED>
-__global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW) void scan_channels_backward_kernel(const ScanParams p, const ScanPlan plan, const int blocks, const long long units) {
-    constexpr int L = backwardSteps(V), GV = SHARED ? 1 : V;
+__global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW, 4) void scan_channels_backward_kernel(const ScanParams p, const ScanPlan plan, const int blocks, const long long units) {
+    constexpr int L = backwardSteps(V, sizeof(T)), GV = SHARED ? 1 : V;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int w = NW == 1 ? 0 : wave;
     const long long unit = NW == 1 ? blockIdx.x * 4LL + wave : blockIdx.x;
@@ -440,26 +436,23 @@ __global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW) void scan_channels_backwar
             T rawG[L][GV], rawX[L][V];
             loadChannels<T, GV, L>(gp, p.gs[1], i0, n, inside, p.reverse, rawG);
             loadChannels<T, V, L>(xp, p.xs[1], i0, n, inside, p.reverse, rawX);
-            float a[L][GV], rest[L][GV], a2[GV], u2[V];
-            gatesOf<T, GV, L>(p, rawG, i0, inside, a, rest);
+            float a2[GV], u2[V];
 #pragma unroll
             for (int v = 0; v < V; ++v) u2[v] = NW == 1 ? at[v] : 0.f;
 #pragma unroll
             for (int v = 0; v < GV; ++v) a2[v] = 1.f;
+            withGates<T, GV, L>(p, rawG, i0, inside, [&](int k, int v, float gate, float factor) {
+                a2[v] *= gate;
 #pragma unroll
-            for (int q = 0; q < L; ++q) {
-#pragma unroll
-                for (int v = 0; v < GV; ++v) a2[v] *= a[q][v];
-#pragma unroll
-                for (int v = 0; v < V; ++v) u2[v] = fmaf(a[q][SHARED ? 0 : v], u2[v], rest[q][SHARED ? 0 : v] * toFloat(rawX[q][v]));
-            }
+                for (int c = SHARED ? 0 : v; c < (SHARED ? V : v + 1); ++c) u2[c] = fmaf(gate, u2[c], factor * toFloat(rawX[k][c]));
+            });
             if constexpr (NW > 1) {
 #pragma unroll
                 for (int v = 0; v < GV; ++v) joined[buffer][w][v][lane] = a2[v];
 #pragma unroll
                 for (int v = 0; v < V; ++v) joined[buffer][w][GV + v][lane] = u2[v];
                 __syncthreads();
-#pragma unroll
+#pragma unroll 2
                 for (int s = 0; s < NW; ++s)
 #pragma unroll
                     for (int v = 0; v < V; ++v) at[v] = fmaf(joined[buffer][s][SHARED ? 0 : v][lane], at[v], joined[buffer][s][GV + v][lane]);
@@ -486,7 +479,10 @@ __global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW) void scan_channels_backwar
                                                                                      : fmaf(heads[(long long)j * p.C + v], h[v], heads[ws.headPlane + (long long)j * p.C + v]);
         }
         float a[L][GV], rest[L][GV], x[L][V], d[L][V], a2[GV], u2[V], d2[V];
-        gatesOf<T, GV, L>(p, rawG, i0, inside, a, rest);
+        withGates<T, GV, L>(p, rawG, i0, inside, [&](int k, int v, float gate, float factor) {
+            a[k][v] = gate;
+            rest[k][v] = factor;
+        });
 #pragma unroll
         for (int v = 0; v < V; ++v) u2[v] = d2[v] = 0.f;
 #pragma unroll
@@ -523,12 +519,11 @@ __global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW) void scan_channels_backwar
             __syncthreads();
 #pragma unroll
             for (int v = 0; v < V; ++v) hw[v] = joined[buffer][0][GV + 2 * V + v][lane];
+#pragma unroll 2
+            for (int s = 0; s < w; ++s)
 #pragma unroll
-            for (int s = 0; s < NW - 1; ++s)
-                if (s < w)
-#pragma unroll
-                    for (int v = 0; v < V; ++v) hw[v] = fmaf(joined[buffer][s][SHARED ? 0 : v][lane], hw[v], joined[buffer][s][GV + v][lane]);
-#pragma unroll
+                for (int v = 0; v < V; ++v) hw[v] = fmaf(joined[buffer][s][SHARED ? 0 : v][lane], hw[v], joined[buffer][s][GV + v][lane]);
+#pragma unroll 2
             for (int s = NW - 1; s >= 0; --s)
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
@@ -1152,7 +1147,7 @@ ScanPlan planScan(const ScanParams& p, int dtype, bool backward) {
         for (int v = most; v > 1 && plan.vec == 1; v >>= 1)
             if (p.C % v == 0 && p.C >= 64 * v) plan.vec = v;
     }
-    const int L = backward ? backwardSteps(plan.vec) : forwardSteps(plan.vec);
+    const int L = backward ? backwardSteps(plan.vec, dtype == FVSRN_TENSOR_F32 ? 4 : 2) : forwardSteps(plan.vec);
     if (backward && p.G > 1 && !plan.shared) {
         plan.slots = std::min(64, powerOfTwoAtLeast(p.G));
         plan.parts = (p.G + 63) / 64;

@@ -20,15 +20,51 @@ typedef int int16_t_ __attribute__((ext_vector_type(16)));
 // Bound by memory: every value is read once and a quarter or half of its bytes written.  `width` lanes share a row, 8 values of each in turn, in registers
 // from the maximum to the codes (of rows longer than 8 width HELD the rest is read a second time, from the caches).  Short rows go ROWS at a time: one
 // 16-byte load a lane would leave the memory idle.  Any alignment: the loads and stores of 8 values are as fast as the lines they touch.
+// The piece that a row's end cuts begins 8 before it instead (what it shares with the piece before is written twice, with the same codes); only rows of less
+// than 8 go value by value.
+__device__ __forceinline__ int pieceAt(int k, int cols) { return min(k, max(cols - 8, 0)); }
+
 template <class T>
 __device__ __forceinline__ void loadEight(const T* row, int k, int cols, T (&v)[8]) {
-    if (k + 8 <= cols) {
-        loadWide<T, 8>(v, row + k);
+    if (cols >= 8) {
+        loadWide<T, 8>(v, row + pieceAt(k, cols));
     } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = k + j < cols ? row[k + j] : T(0.f);
+        for (int j = 0; j < 8; ++j) v[j] = j < cols ? row[j] : T(0.f);
     }
 }
+
+// The largest magnitude of pairs of values, by their bits: without its sign a float is ordered like its bits, and what is no finite number is above all others.
+template <class T>
+struct Largest {
+    typedef unsigned word;
+    static constexpr unsigned kInfinity = 0x7f800000u;
+    word most = 0;
+    __device__ __forceinline__ void look(const T (&v)[8]) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) most = max(most, __float_as_uint(v[j]) & 0x7fffffffu);
+    }
+    __device__ __forceinline__ unsigned key() const { return most; }
+    static __device__ __forceinline__ float value(unsigned key) { return __uint_as_float(key); }
+};
+template <class T>
+struct Largest16 {
+    typedef unsigned short word __attribute__((ext_vector_type(2)));
+    word most = {0, 0};
+    __device__ __forceinline__ void look(const T (&v)[8]) {
+        const word sign = {0x7fff, 0x7fff};
+        word w[4];
+        __builtin_memcpy(w, v, 16);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) most = __builtin_elementwise_max(most, w[j] & sign);
+    }
+    __device__ __forceinline__ unsigned key() const { return max(most.x, most.y); }
+    static __device__ __forceinline__ float value(unsigned key) { return toFloat(__builtin_bit_cast(T, (unsigned short)key)); }
+};
+template <>
+struct Largest<f16_t> : Largest16<f16_t> { static constexpr unsigned kInfinity = 0x7c00u; };
+template <>
+struct Largest<bf16_t> : Largest16<bf16_t> { static constexpr unsigned kInfinity = 0x7f80u; };
 
 // The codes are the quotients v / scale rounded to 32 bits, rounded to integers.  A division is ten instructions, and they would be what the kernel waits for: where it
 // can be, the quotient is q = v y with y = 1 / scale rounded, corrected by its exact remainder, q + (v - q scale) y, which is the rounded quotient
@@ -48,12 +84,12 @@ __device__ __forceinline__ void storeEight(signed char* row, int k, int cols, co
         const unsigned lo = __builtin_amdgcn_perm(w[4 * j + 1], w[4 * j], 0x0c0c0400u), hi = __builtin_amdgcn_perm(w[4 * j + 3], w[4 * j + 2], 0x04000c0cu);
         word[j] = zero ? 0u : lo | hi;
     }
-    if (k + 8 <= cols) {
-        storeWide<signed char, 8>(row + k, reinterpret_cast<const signed char*>(word));
+    if (cols >= 8) {
+        storeWide<signed char, 8>(row + pieceAt(k, cols), reinterpret_cast<const signed char*>(word));
     } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-            if (k + j < cols) row[k + j] = (signed char)(word[j >> 2] >> (8 * (j & 3)));
+            if (j < cols) row[j] = (signed char)(word[j >> 2] >> (8 * (j & 3)));
     }
 }
 
@@ -72,29 +108,20 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const QuantizeParams
     for (int r = 0; r < ROWS; ++r) {
         const long long row = min(first + r * groups, p.rows - 1);
         const T* const x = static_cast<const T*>(p.x) + row * p.ldx;
-        float most = 0.f, odd = 0.f;
-        auto look = [&](const T(&w)[8]) {
+        Largest<T> largest;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                most = fmaxf(most, fabsf(toFloat(w[e])));
-                odd = fmaf(toFloat(w[e]), 0.f, odd);  // (NaN once a value is no finite number)
-            }
-        };
-#pragma unroll
-        for (int j = 0; j < HELD; ++j) look(v[r][j]);
+        for (int j = 0; j < HELD; ++j) largest.look(v[r][j]);
         for (int k = (HELD * width + at) * 8; k < p.cols; k += width * 8) {
             T w[8];
             loadEight(x, k, p.cols, w);
-            look(w);
+            largest.look(w);
         }
-        for (int o = 1; o < width; o <<= 1) {
-            most = fmaxf(most, __shfl_xor(most, o, 64));
-            odd += __shfl_xor(odd, o, 64);
-        }
+        unsigned key = largest.key();
+        for (int o = 1; o < width; o <<= 1) key = max(key, __shfl_xor(key, o, 64));
         if (first + r * groups >= p.rows) return;
-        const bool bad = odd != odd;
+        const bool bad = key >= Largest<T>::kInfinity;
         signed char* const q = p.codes + row * p.ldc;
-        const float scale = fmaxf(most * (1.f / 127.f), 0x1p-126f);
+        const float scale = fmaxf(Largest<T>::value(key) * (1.f / 127.f), 0x1p-126f);
         if (at == 0) p.scales[row] = bad ? __builtin_nanf("") : scale;
         const float y = __fdiv_rn(1.f, scale);
         const bool exact = scale > 0x1p-90f && (__float_as_uint(scale) & 0x7fffffu) != 0x7fffffu;
@@ -170,20 +197,31 @@ __device__ __forceinline__ void withActivation(int kind, F&& f) {
 // Sums of products are exact whatever their order, so k may be cut and joined anywhere.
 
 // 16 bytes of a row from column k, zeros behind its end.  ALIGNED: k and the row start are multiples of 16 (and so is K: no chunk is cut); otherwise one unaligned
-// load, which costs what the lines it touches cost, and single bytes at the row's end.
+// load, which costs what the lines it touches cost; a chunk that the row's end cuts is the row's last 16 bytes shifted down.
 template <bool ALIGNED>
 __device__ __forceinline__ int4_t loadCodes(const signed char* row, int k, int K) {
-    if (k + 16 <= K) {
-        if (ALIGNED) return *reinterpret_cast<const int4_t*>(row + k);
-        int4_t v;
-        __builtin_memcpy(&v, row + k, 16);
+    typedef unsigned long long word_t;
+    const int4_t none = {0, 0, 0, 0};
+    if (ALIGNED) return k < K ? *reinterpret_cast<const int4_t*>(row + k) : none;
+    if (k >= K) return none;
+    if (K < 16) {
+        int4_t v = none;
+#pragma unroll
+        for (int j = 0; j < 15; ++j)
+            if (j < K) v[j >> 2] |= int(static_cast<unsigned char>(row[j])) << (8 * (j & 3));
         return v;
     }
-    int4_t v = {0, 0, 0, 0};
-    if (ALIGNED) return v;
-#pragma unroll
-    for (int j = 0; j < 16; ++j)
-        if (k + j < K) v[j >> 2] |= int(static_cast<unsigned char>(row[k + j])) << (8 * (j & 3));
+    int4_t v;
+    __builtin_memcpy(&v, row + min(k, K - 16), 16);
+    if (k + 16 <= K) return v;
+    const int bits = 8 * (k + 16 - K);  // 8 .. 120
+    word_t lo, hi;
+    __builtin_memcpy(&lo, &v, 8);
+    __builtin_memcpy(&hi, reinterpret_cast<const char*>(&v) + 8, 8);
+    lo = bits >= 64 ? hi >> (bits & 63) : lo >> bits | hi << (64 - bits);
+    hi = bits >= 64 ? 0 : hi >> bits;
+    __builtin_memcpy(&v, &lo, 8);
+    __builtin_memcpy(reinterpret_cast<char*>(&v) + 8, &hi, 8);
     return v;
 }
 
@@ -243,61 +281,75 @@ __global__ __launch_bounds__(512) void matmul_int8_few_kernel(const Int8Params p
     }
 }
 
-// Any alignment: v_mfma_i32_32x32x32_i8, lane l holds 16 consecutive k (half l / 32) of row l % 32 of either operand; register r of the result is row
-// 8 (r / 4) + 4 (l / 32) + r % 4, column l % 32.  One workgroup: 64 tokens x 64 channels, four waves of 32 x 32.
+// Few channels (the last layer of a network) for many tokens: bound by the tokens' bytes.  The same instruction with the same operands -- 16 channels as its rows, 16
+// tokens as its columns, a lane's four results four channels of one token -- but a wave takes 64 tokens through all of k, and nothing is joined.
 template <class T, bool ALIGNED>
-__global__ __launch_bounds__(256) void matmul_int8_kernel(const Int8Params p, const int activation) {
-    constexpr int S = 80;  // LDS row: 64 bytes of k and 16 of padding
-    __shared__ __attribute__((aligned(16))) signed char as[64 * S], bs[64 * S];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const long long m0 = blockIdx.x * 64LL;
-    const int n0 = blockIdx.y * 64;
-    const int lr = tid >> 2, lk = (tid & 3) * 16;
-    const signed char* const ar = p.a + min(m0 + lr, p.M - 1) * p.lda;
-    const signed char* const br = p.b + (long long)min(n0 + lr, p.N - 1) * p.ldb;
-    const int wm = (wave >> 1) * 32, wn = (wave & 1) * 32, col = lane & 31, half = lane >> 5;
-    int16_t_ acc = {};
-    for (int k0 = 0; k0 < p.K; k0 += 64) {
-        const int4_t av = loadCodes<ALIGNED>(ar, k0 + lk, p.K), bv = loadCodes<ALIGNED>(br, k0 + lk, p.K);
-        __syncthreads();
-        *reinterpret_cast<int4_t*>(as + lr * S + lk) = av;
-        *reinterpret_cast<int4_t*>(bs + lr * S + lk) = bv;
-        __syncthreads();
+__global__ __launch_bounds__(256) void matmul_int8_narrow_kernel(const Int8Params p, const int activation) {
+    constexpr int GROUPS = 4;
+    const int lane = threadIdx.x & 63, col = lane & 15, part = lane >> 4;
+    const long long m0 = (blockIdx.x * 4LL + (threadIdx.x >> 6)) * (16 * GROUPS);
+    if (m0 >= p.M) return;
+    const signed char* const br = p.b + (long long)min(col, p.N - 1) * p.ldb;
+    const signed char* ar[GROUPS];
 #pragma unroll
-        for (int kk = 0; kk < 64; kk += 32) {
-            const int4_t a = *reinterpret_cast<const int4_t*>(as + (wm + col) * S + kk + half * 16);
-            const int4_t b = *reinterpret_cast<const int4_t*>(bs + (wn + col) * S + kk + half * 16);
-            acc = __builtin_amdgcn_mfma_i32_32x32x32_i8(a, b, acc, 0, 0, 0);
-        }
+    for (int t = 0; t < GROUPS; ++t) ar[t] = p.a + min(m0 + t * 16 + col, p.M - 1) * p.lda;
+    int4_t acc[GROUPS] = {};
+#pragma unroll 2
+    for (int k = part * 16; k < p.K + part * 16; k += 64) {  // (as many steps for every lane)
+        const int4_t b = loadCodes<ALIGNED>(br, k, p.K);
+        int4_t a[GROUPS];
+#pragma unroll
+        for (int t = 0; t < GROUPS; ++t) a[t] = loadCodes<ALIGNED>(ar[t], k, p.K);
+#pragma unroll
+        for (int t = 0; t < GROUPS; ++t) acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(b, a[t], acc[t], 0, 0, 0);
     }
-    const int n = n0 + wn + col;
+    const int n = part * 4;
     if (n >= p.N) return;
-    const float sb = p.scaleB[n], bias = p.bias ? p.bias[n] : 0.f;
-    float sa[16];
+    float sb[4], bias[4];
 #pragma unroll
-    for (int r = 0; r < 16; ++r) sa[r] = p.scaleA[min(m0 + wm + 8 * (r >> 2) + 4 * half + (r & 3), p.M - 1)];
+    for (int r = 0; r < 4; ++r) {
+        const int c = min(n + r, p.N - 1);
+        sb[r] = p.scaleB[c];
+        bias[r] = p.bias ? p.bias[c] : 0.f;
+    }
     withActivation(activation, [&](auto kind) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            const long long m = m0 + wm + 8 * (r >> 2) + 4 * half + (r & 3);
-            if (m < p.M) static_cast<T*>(p.out)[m * p.ldo + n] = fromFloat<T>(scaled<decltype(kind)::value>(acc[r], sa[r], sb, bias, p.actParam));
+        for (int t = 0; t < GROUPS; ++t) {
+            const long long m = m0 + t * 16 + col;
+            if (m >= p.M) continue;
+            const float sa = p.scaleA[m];
+            T o[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) o[r] = fromFloat<T>(scaled<decltype(kind)::value>(acc[t][r], sa, sb[r], bias[r], p.actParam));
+            T* const out = static_cast<T*>(p.out) + m * p.ldo + n;
+            if (n + 4 <= p.N) {
+                storeWide<T, 4>(out, o);
+            } else {
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (n + r < p.N) out[r] = o[r];
+            }
         }
     });
 }
 
-// Aligned rows: a tile of TM tokens x TN channels for WM x WN waves, each with PM x 2 pieces of 32 x 32, 64 bytes of k a stage.
+// A tile of TM tokens x TN channels for WM x WN waves, each with PM x 2 pieces of 32 x 32, 64 bytes of k a stage.  v_mfma_i32_32x32x32_i8: lane l holds 16
+// consecutive k (half l / 32) of row l % 32 of either operand; register r of the result is row 8 (r / 4) + 4 (l / 32) + r % 4, column l % 32.
 //   Stages go from memory into LDS without passing a register, into a ring of RING: while one is multiplied the others travel (a stage of 256 x 256 is multiplied in
 // 0.4 us, which is less than the way from memory).  The wait for the next stage and the barrier stand between the two halves of a stage's products, and the
 // operands of a half are read while the half before is multiplied, so the matrix units have work queued at every wait.
+//   Not DIRECT (rows that are not aligned to 16 bytes): a stage goes through registers, asked for a stage ahead of its way into a ring of two -- unaligned addresses
+// are for registers only, and so is the masking of the chunk in which K ends.
 //   LDS holds rows of four 16-byte chunks, chunk c of row r at place c ^ swizzle(r), so that the 32 rows a wave reads at one k spread over all banks; the
 // loads write LDS in lane order, so it is their source that is permuted.  A wave's channels are paired -- column l of its piece j is channel 2 l + j -- so that a
 // lane stores two adjacent outputs and a wave whole 128-byte lines of 16-bit ones.
-template <class T, int TM, int TN, int WM, int WN, int RING>
+template <class T, int TM, int TN, int WM, int WN, int RING, bool DIRECT>
 __global__ __launch_bounds__(64 * WM * WN) void matmul_int8_tile_kernel(const Int8Params p, const int activation, const int tilesM, const int tilesN) {
     constexpr int BK = 64, WAVES = WM * WN, PM = TM / WM / 32, STAGE = (TM + TN) * BK;
     static_assert(TN / WN == 64, "a wave's channels are paired");
     constexpr int LOADS = STAGE / 1024 / WAVES;  // of a wave, 1 KiB each: 16 rows
     static_assert(STAGE % (1024 * WAVES) == 0 && LOADS * (RING - 2) < 64, "the waits below count loads");
+    static_assert(DIRECT || RING == 2, "through registers two buffers do");
     constexpr int FLOWING = LOADS * (RING - 2);  // loads that may still be on their way when the next stage is waited for
     __shared__ __attribute__((aligned(1024))) signed char lds[RING][STAGE];
     __shared__ __attribute__((aligned(16))) float scaleA[TM], scaleB[TN], bias[TN];
@@ -316,9 +368,18 @@ __global__ __launch_bounds__(64 * WM * WN) void matmul_int8_tile_kernel(const In
         const int row = (wave * LOADS + j) * 16 + (lane >> 2);  // of the tile: tokens, then channels
         const bool token = row < TM;
         chunk[j] = ((lane & 3) ^ ((token ? row >> 1 : row >> 2) & 3)) * 16;
-        source[j] = (token ? p.a + min(m0 + row, p.M - 1) * p.lda : p.b + (long long)min(n0 + row - TM, p.N - 1) * p.ldb) + chunk[j];
+        source[j] = (token ? p.a + min(m0 + row, p.M - 1) * p.lda : p.b + (long long)min(n0 + row - TM, p.N - 1) * p.ldb) + (DIRECT ? chunk[j] : 0);
     }
     const int stages = (p.K + BK - 1) / BK;
+    int4_t staged[LOADS];
+    auto fetch = [&](int stage) {
+#pragma unroll
+        for (int j = 0; j < LOADS; ++j) staged[j] = loadCodes<false>(source[j], stage * BK + chunk[j], p.K);
+    };
+    auto put = [&](int stage) {
+#pragma unroll
+        for (int j = 0; j < LOADS; ++j) *reinterpret_cast<int4_t*>(&lds[stage % RING][(wave * LOADS + j) * 1024 + lane * 16]) = staged[j];
+    };
     auto load = [&](int stage) {
 #pragma unroll
         for (int j = 0; j < LOADS; ++j) {
@@ -364,18 +425,38 @@ __global__ __launch_bounds__(64 * WM * WN) void matmul_int8_tile_kernel(const In
         else __builtin_amdgcn_s_waitcnt(0x0070);                                                  // vmcnt(0) lgkmcnt(0)
         asm volatile("s_barrier" ::: "memory");
     };
-    for (int s = 0; s < min(RING - 1, stages); ++s) load(s);
-    arrive(stages >= RING - 1);
     Operands even, odd;
-    read(even, 0, 0);
+    if constexpr (DIRECT) {
+        for (int s = 0; s < min(RING - 1, stages); ++s) load(s);
+        arrive(stages >= RING - 1);
+        read(even, 0, 0);
 #pragma unroll 1
-    for (int s = 0; s < stages - 1; ++s) {
-        if (s + RING - 1 < stages) load(s + RING - 1);
-        read(odd, s, 1);
-        multiply(even);
-        arrive(s + RING - 1 < stages);
-        read(even, s + 1, 0);
-        multiply(odd);
+        for (int s = 0; s < stages - 1; ++s) {
+            if (s + RING - 1 < stages) load(s + RING - 1);
+            read(odd, s, 1);
+            multiply(even);
+            arrive(s + RING - 1 < stages);
+            read(even, s + 1, 0);
+            multiply(odd);
+        }
+    } else {
+        fetch(0);
+        put(0);
+        if (stages > 1) fetch(1);
+        __syncthreads();
+        read(even, 0, 0);
+#pragma unroll 1
+        for (int s = 0; s < stages - 1; ++s) {
+            put(s + 1);  // (nobody reads stage s - 1 any more since the last barrier)
+            if (s + 2 < stages) fetch(s + 2);
+            read(odd, s, 1);
+            multiply(even);
+            // (lgkmcnt(0) only: what was fetched stays on its way)
+            __builtin_amdgcn_s_waitcnt(0xc07f);
+            asm volatile("s_barrier" ::: "memory");
+            read(even, s + 1, 0);
+            multiply(odd);
+        }
     }
     // the last stage: zeros in the place of what lies behind K
     read(odd, stages - 1, 1);
@@ -443,7 +524,8 @@ hipError_t withType(int dtype, F&& f) {
 hipError_t launch_quantize_rows(const QuantizeParams& p, int dtype, hipStream_t s) {
     return withType(dtype, [&](auto element) {
         typedef decltype(element) T;
-        const int width = std::min(64, powerOfTwoAtLeast((p.cols + 7) / 8));
+        // 16 values of a lane in rows of up to 1024: what a row costs beside its values -- the maximum's way through the lanes, the reciprocal -- is spread over them
+        const int width = std::min(64, powerOfTwoAtLeast(p.cols <= 1024 ? (p.cols + 15) / 16 : (p.cols + 7) / 8));
         auto launch = [&](auto held, auto rows) {
             constexpr int H = decltype(held)::value, R = decltype(rows)::value;
             const long long rowsOfBlock = 4 * (64 / width) * R;
@@ -451,8 +533,8 @@ hipError_t launch_quantize_rows(const QuantizeParams& p, int dtype, hipStream_t 
             return hipGetLastError();
         };
         // (rows at a time: only where there are enough of them for 8 waves on each CU all the same)
-        if (p.cols <= 512 && p.rows * width >= 4LL * 64 * 2048) return launch(std::integral_constant<int, 1>{}, std::integral_constant<int, 4>{});
-        if (p.cols <= 512) return launch(std::integral_constant<int, 1>{}, std::integral_constant<int, 1>{});
+        if (p.cols <= 1024 && p.rows * width >= 4LL * 64 * 2048) return launch(std::integral_constant<int, 2>{}, std::integral_constant<int, 4>{});
+        if (p.cols <= 1024) return launch(std::integral_constant<int, 2>{}, std::integral_constant<int, 1>{});
         if (p.cols <= 2048) return launch(std::integral_constant<int, 4>{}, std::integral_constant<int, 1>{});
         return launch(std::integral_constant<int, 8>{}, std::integral_constant<int, 1>{});
     });
@@ -474,24 +556,26 @@ hipError_t launch_matmul_int8(const Int8Params& p, int activation, int outDtype,
             return few(isAligned, std::integral_constant<int, 4>{});
         };
         if (p.M <= 64) return aligned ? fewOf(std::true_type{}) : fewOf(std::false_type{});
-        auto tiles = [&](int edge) { return ((p.M + edge - 1) / edge) * ((p.N + edge - 1) / edge); };
-        if (aligned && p.N > 32 && tiles(64) < (1LL << 24)) {
-            // The largest tile that still gives every CU one (edges of 256 only with k long enough to hide their beginning and end: one fits a CU). 8192 x
-            // 4096 x 4096: 145 us with 256, 199 with 128, 300 with 64; 262144 x 256 x 256: 46, 43, 61 us; 2048 x 1024 x 1024: 16, 10, 9 us.
-            auto launch = [&](auto edge, auto wavesM, auto wavesN, auto ring) {
-                constexpr int E = decltype(edge)::value, WM = decltype(wavesM)::value, WN = decltype(wavesN)::value;
-                matmul_int8_tile_kernel<T, E, E, WM, WN, decltype(ring)::value><<<unsigned(tiles(E)), 64 * WM * WN, 0, s>>>(p, activation, int((p.M + E - 1) / E), (p.N + E - 1) / E);
-            };
-            using std::integral_constant;
-            if (tiles(256) >= 256 && p.K >= 1024) launch(integral_constant<int, 256>{}, integral_constant<int, 4>{}, integral_constant<int, 4>{}, integral_constant<int, 3>{});
-            else if (tiles(128) >= 256) launch(integral_constant<int, 128>{}, integral_constant<int, 2>{}, integral_constant<int, 2>{}, integral_constant<int, 3>{});
-            else launch(integral_constant<int, 64>{}, integral_constant<int, 2>{}, integral_constant<int, 1>{}, integral_constant<int, 4>{});
+        if (p.N <= 16) {
+            const unsigned grid = unsigned((p.M + 255) / 256);
+            if (aligned) matmul_int8_narrow_kernel<T, true><<<grid, 256, 0, s>>>(p, activation);
+            else matmul_int8_narrow_kernel<T, false><<<grid, 256, 0, s>>>(p, activation);
             return hipGetLastError();
         }
-        const dim3 grid(unsigned((p.M + 63) / 64), unsigned((p.N + 63) / 64));
-        if (aligned) matmul_int8_kernel<T, true><<<grid, 256, 0, s>>>(p, activation);
-        else matmul_int8_kernel<T, false><<<grid, 256, 0, s>>>(p, activation);
-        return hipGetLastError();
+        // The largest tile that still gives every CU one (edges of 256 only with k long enough to hide their beginning and end: one fits a CU). 8192 x 4096 x 4096: 145
+        // us with 256, 199 with 128, 300 with 64; 262144 x 256 x 256: 46, 43, 61 us; 2048 x 1024 x 1024: 16, 10, 9 us.
+        auto tiles = [&](int edge) { return ((p.M + edge - 1) / edge) * ((p.N + edge - 1) / edge); };
+        auto launch = [&](auto edge, auto wavesM, auto wavesN, auto ring) {
+            constexpr int E = decltype(edge)::value, WM = decltype(wavesM)::value, WN = decltype(wavesN)::value, R = decltype(ring)::value;
+            const int tilesM = int((p.M + E - 1) / E), tilesN = (p.N + E - 1) / E;
+            if (aligned) matmul_int8_tile_kernel<T, E, E, WM, WN, R, true><<<unsigned(tiles(E)), 64 * WM * WN, 0, s>>>(p, activation, tilesM, tilesN);
+            else matmul_int8_tile_kernel<T, E, E, WM, WN, 2, false><<<unsigned(tiles(E)), 64 * WM * WN, 0, s>>>(p, activation, tilesM, tilesN);
+            return hipGetLastError();
+        };
+        using std::integral_constant;
+        if (tiles(256) >= 256 && p.K >= 1024) return launch(integral_constant<int, 256>{}, integral_constant<int, 4>{}, integral_constant<int, 4>{}, integral_constant<int, 3>{});
+        if (tiles(128) >= 256) return launch(integral_constant<int, 128>{}, integral_constant<int, 2>{}, integral_constant<int, 2>{}, integral_constant<int, 3>{});
+        return launch(integral_constant<int, 64>{}, integral_constant<int, 2>{}, integral_constant<int, 1>{}, integral_constant<int, 4>{});
     });
 }
 
