@@ -147,7 +147,7 @@ __device__ __forceinline__ void withGates(const ScanParams& p, const T (&raw)[L]
 template <class T, int NW, int V, bool SHARED, bool AGGREGATE>
 __global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW) void scan_channels_kernel(const ScanParams p, const ScanPlan plan, const int blocks, const long long units) {
     constexpr int L = forwardSteps(V), GV = SHARED ? 1 : V;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // (known to be the same for a wave: its addresses are scalars)
     const int w = NW == 1 ? 0 : wave;
     const long long unit = NW == 1 ? blockIdx.x * 4LL + wave : blockIdx.x;
     if (unit >= units) return;  // (NW == 1 only, and nothing is joined across its waves)
@@ -299,7 +299,7 @@ inline size_t backwardFloats(const ScanParams& p, const ScanPlan& plan) {
 template <class T, int NW, int V, bool SHARED>
 __global__ __launch_bounds__(64 * NW) void scan_channels_spans_kernel(const ScanParams p, const ScanPlan plan, const int blocks) {
     constexpr int L = backwardSteps(V, sizeof(T)), GV = SHARED ? 1 : V;
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const long long b = blockIdx.x / blocks;
     const ChannelLane ch = channelLane<V, SHARED>(p, int(blockIdx.x % blocks), lane, plan.slots, plan.parts);
     const int n = lengthOf(p, b), span = blockIdx.y;
@@ -381,7 +381,7 @@ __global__ __launch_bounds__(64 * NW) void scan_channels_spans_kernel(const Scan
 template <class T, int NW, int V, bool SHARED>
 __global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW, 4) void scan_channels_backward_kernel(const ScanParams p, const ScanPlan plan, const int blocks, const long long units) {
     constexpr int L = backwardSteps(V, sizeof(T)), GV = SHARED ? 1 : V;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // (known to be the same for a wave: its addresses are scalars)
     const int w = NW == 1 ? 0 : wave;
     const long long unit = NW == 1 ? blockIdx.x * 4LL + wave : blockIdx.x;
     if (unit >= units) return;

@@ -196,34 +196,67 @@ __device__ __forceinline__ void withActivation(int kind, F&& f) {
 
 // Sums of products are exact whatever their order, so k may be cut and joined anywhere.
 
-// 16 bytes of a row from column k, zeros behind its end.  ALIGNED: k and the row start are multiples of 16 (and so is K: no chunk is cut); otherwise one unaligned
-// load, which costs what the lines it touches cost; a chunk that the row's end cuts is the row's last 16 bytes shifted down.
-template <bool ALIGNED>
-__device__ __forceinline__ int4_t loadCodes(const signed char* row, int k, int K) {
-    typedef unsigned long long word_t;
-    const int4_t none = {0, 0, 0, 0};
-    if (ALIGNED) return k < K ? *reinterpret_cast<const int4_t*>(row + k) : none;
-    if (k >= K) return none;
-    if (K < 16) {
-        int4_t v = none;
-#pragma unroll
-        for (int j = 0; j < 15; ++j)
-            if (j < K) v[j >> 2] |= int(static_cast<unsigned char>(row[j])) << (8 * (j & 3));
-        return v;
-    }
+// 16 bytes of a row from column k, zeros behind the row's end, in two steps so that many loads are on their way before the first is looked at.
+//   kAligned: k and the row start are multiples of 16, and so is K: no chunk is cut, and one behind the end (the row's start is read for it) is dropped.
+//   Otherwise the row's last 16 bytes are read where the chunk reaches behind its end, and shifted down: in one load at whatever address (kBytes), or as the five
+// aligned words that hold them (kWords).  An odd address makes a load several times as long, a fifth word a quarter: with few waves on the way through k the words win
+// (64 x 4096 x 4095 20 against 39 us, 100003 x 4 x 250 10 against 13), in tiles, which wait for LDS and not for these, the single load (8192 x
+// 4096 x 4095 160 against 204 us).  A word is read only if one of its bytes is the row's, and an aligned word never leaves a page, so nothing is touched that the
+// row does not share with its neighbours.
+enum CodeLoads { kAligned, kWords, kBytes };
+template <CodeLoads HOW>
+struct Codes {
+    static constexpr bool ALIGNED = HOW == kAligned;
     int4_t v;
-    __builtin_memcpy(&v, row + min(k, K - 16), 16);
-    if (k + 16 <= K) return v;
-    const int bits = 8 * (k + 16 - K);  // 8 .. 120
-    word_t lo, hi;
-    __builtin_memcpy(&lo, &v, 8);
-    __builtin_memcpy(&hi, reinterpret_cast<const char*>(&v) + 8, 8);
-    lo = bits >= 64 ? hi >> (bits & 63) : lo >> bits | hi << (64 - bits);
-    hi = bits >= 64 ? 0 : hi >> bits;
-    __builtin_memcpy(&v, &lo, 8);
-    __builtin_memcpy(reinterpret_cast<char*>(&v) + 8, &hi, 8);
-    return v;
-}
+    unsigned w;
+
+    static __device__ __forceinline__ const signed char* start(const signed char* row, int k, int K) { return row + min(k, max(K - 16, 0)); }
+
+    __device__ __forceinline__ void load(const signed char* row, int k, int K) {
+        if (ALIGNED) {
+            v = *reinterpret_cast<const int4_t*>(row + (k < K ? k : 0));
+        } else if (K >= 16 && HOW == kBytes) {
+            __builtin_memcpy(&v, start(row, k, K), 16);
+        } else if (K >= 16) {
+            const size_t at = reinterpret_cast<size_t>(start(row, k, K));
+            const unsigned* const words = reinterpret_cast<const unsigned*>(at & ~size_t(3));
+            unsigned from[4];
+            loadWide<unsigned, 4>(from, words);
+            __builtin_memcpy(&v, from, 16);
+            w = words[at & 3 ? 4 : 3];
+        } else {
+            v = int4_t{0, 0, 0, 0};
+#pragma unroll
+            for (int j = 0; j < 15; ++j)
+                if (j < K) v[j >> 2] |= int(static_cast<unsigned char>(row[j])) << (8 * (j & 3));
+        }
+    }
+
+    // cut: whether K may end in or before this chunk
+    __device__ __forceinline__ int4_t get(const signed char* row, int k, int K, bool cut) const {
+        if (ALIGNED || K < 16) return !cut || k < K ? v : int4_t{0, 0, 0, 0};
+        typedef unsigned long long word_t;
+        unsigned u[4];
+        if (HOW == kWords) {
+            const unsigned odd = unsigned(reinterpret_cast<size_t>(start(row, k, K))) & 3;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) u[j] = __builtin_amdgcn_alignbyte(j < 3 ? unsigned(v[j + 1]) : w, unsigned(v[j]), odd);
+        } else {
+            __builtin_memcpy(u, &v, 16);
+        }
+        if (cut) {
+            const int bits = 8 * max(0, k + 16 - K);  // how far the load began before k: below 128 in a chunk that has bytes of the row
+            const word_t lo = u[0] | word_t(u[1]) << 32, hi = u[2] | word_t(u[3]) << 32;
+            const word_t low = bits >= 128 ? 0 : bits >= 64 ? hi >> (bits & 63) : bits > 0 ? lo >> bits | hi << (64 - bits) : lo;
+            const word_t high = bits >= 64 ? 0 : hi >> bits;
+            u[0] = unsigned(low);
+            u[1] = unsigned(low >> 32);
+            u[2] = unsigned(high);
+            u[3] = unsigned(high >> 32);
+        }
+        return int4_t{int(u[0]), int(u[1]), int(u[2]), int(u[3])};
+    }
+};
 
 template <int KIND>
 __device__ __forceinline__ float scaled(int acc, float sa, float sb, float bias, float param) {
@@ -234,7 +267,7 @@ __device__ __forceinline__ float scaled(int acc, float sa, float sb, float bias,
 // consecutive k (part l / 16) of channel l % 16 and of token l % 16; register r of the result is channel 4 (l / 16) + r, token l % 16.  A workgroup has 16 channels and 16 MT
 // tokens; its eight waves take every eighth 256 bytes of k straight from memory into registers -- each weight is read once by the chip, nothing is
 // worth a turn through LDS but the eight sums at the end.
-template <class T, bool ALIGNED, int MT>
+template <class T, CodeLoads HOW, int MT>
 __global__ __launch_bounds__(512) void matmul_int8_few_kernel(const Int8Params p, const int activation) {
     constexpr int W = 8, U = 4;
     __shared__ int4_t sums[W][MT][64];
@@ -247,18 +280,26 @@ __global__ __launch_bounds__(512) void matmul_int8_few_kernel(const Int8Params p
     for (int t = 0; t < MT; ++t) ar[t] = p.a + min(m0 + t * 16 + col, p.M - 1) * p.lda;
     int4_t acc[MT] = {};
     for (int k0 = wave * 64 * U; k0 < p.K; k0 += W * 64 * U) {
-        int4_t b[U], a[MT][U];
+        Codes<HOW> b[U], a[MT][U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int k = k0 + u * 64 + part * 16;
-            b[u] = loadCodes<ALIGNED>(br, k, p.K);
+            b[u].load(br, k, p.K);
 #pragma unroll
-            for (int t = 0; t < MT; ++t) a[t][u] = loadCodes<ALIGNED>(ar[t], k, p.K);
+            for (int t = 0; t < MT; ++t) a[t][u].load(ar[t], k, p.K);
         }
+        // (the same for all lanes; both operands are cut: what lies behind K in one is not 0 in the other)
+        auto multiply = [&](bool cut) {
 #pragma unroll
-        for (int u = 0; u < U; ++u)
+            for (int u = 0; u < U; ++u) {
+                const int k = k0 + u * 64 + part * 16;
+                const int4_t bu = b[u].get(br, k, p.K, cut);
 #pragma unroll
-            for (int t = 0; t < MT; ++t) acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(b[u], a[t][u], acc[t], 0, 0, 0);
+                for (int t = 0; t < MT; ++t) acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(bu, a[t][u].get(ar[t], k, p.K, cut), acc[t], 0, 0, 0);
+            }
+        };
+        if (k0 + 64 * U > p.K) multiply(true);
+        else multiply(false);
     }
 #pragma unroll
     for (int t = 0; t < MT; ++t) sums[wave][t][lane] = acc[t];
@@ -283,7 +324,7 @@ __global__ __launch_bounds__(512) void matmul_int8_few_kernel(const Int8Params p
 
 // Few channels (the last layer of a network) for many tokens: bound by the tokens' bytes.  The same instruction with the same operands -- 16 channels as its rows, 16
 // tokens as its columns, a lane's four results four channels of one token -- but a wave takes 64 tokens through all of k, and nothing is joined.
-template <class T, bool ALIGNED>
+template <class T, CodeLoads HOW>
 __global__ __launch_bounds__(256) void matmul_int8_narrow_kernel(const Int8Params p, const int activation) {
     constexpr int GROUPS = 4;
     const int lane = threadIdx.x & 63, col = lane & 15, part = lane >> 4;
@@ -296,12 +337,14 @@ __global__ __launch_bounds__(256) void matmul_int8_narrow_kernel(const Int8Param
     int4_t acc[GROUPS] = {};
 #pragma unroll 2
     for (int k = part * 16; k < p.K + part * 16; k += 64) {  // (as many steps for every lane)
-        const int4_t b = loadCodes<ALIGNED>(br, k, p.K);
-        int4_t a[GROUPS];
+        Codes<HOW> b, a[GROUPS];
+        b.load(br, k, p.K);
 #pragma unroll
-        for (int t = 0; t < GROUPS; ++t) a[t] = loadCodes<ALIGNED>(ar[t], k, p.K);
+        for (int t = 0; t < GROUPS; ++t) a[t].load(ar[t], k, p.K);
+        const bool cut = k - part * 16 + 64 > p.K;
+        const int4_t bk = b.get(br, k, p.K, cut);
 #pragma unroll
-        for (int t = 0; t < GROUPS; ++t) acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(b, a[t], acc[t], 0, 0, 0);
+        for (int t = 0; t < GROUPS; ++t) acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(bk, a[t].get(ar[t], k, p.K, cut), acc[t], 0, 0, 0);
     }
     const int n = part * 4;
     if (n >= p.N) return;
@@ -371,14 +414,15 @@ __global__ __launch_bounds__(64 * WM * WN) void matmul_int8_tile_kernel(const In
         source[j] = (token ? p.a + min(m0 + row, p.M - 1) * p.lda : p.b + (long long)min(n0 + row - TM, p.N - 1) * p.ldb) + (DIRECT ? chunk[j] : 0);
     }
     const int stages = (p.K + BK - 1) / BK;
-    int4_t staged[LOADS];
+    Codes<kBytes> staged[LOADS];
     auto fetch = [&](int stage) {
 #pragma unroll
-        for (int j = 0; j < LOADS; ++j) staged[j] = loadCodes<false>(source[j], stage * BK + chunk[j], p.K);
+        for (int j = 0; j < LOADS; ++j) staged[j].load(source[j], stage * BK + chunk[j], p.K);
     };
-    auto put = [&](int stage) {
+    auto put = [&](int stage, bool cut) {
 #pragma unroll
-        for (int j = 0; j < LOADS; ++j) *reinterpret_cast<int4_t*>(&lds[stage % RING][(wave * LOADS + j) * 1024 + lane * 16]) = staged[j];
+        for (int j = 0; j < LOADS; ++j)
+            *reinterpret_cast<int4_t*>(&lds[stage % RING][(wave * LOADS + j) * 1024 + lane * 16]) = staged[j].get(source[j], stage * BK + chunk[j], p.K, cut);
     };
     auto load = [&](int stage) {
 #pragma unroll
@@ -441,13 +485,15 @@ __global__ __launch_bounds__(64 * WM * WN) void matmul_int8_tile_kernel(const In
         }
     } else {
         fetch(0);
-        put(0);
+        put(0, true);
         if (stages > 1) fetch(1);
         __syncthreads();
         read(even, 0, 0);
 #pragma unroll 1
         for (int s = 0; s < stages - 1; ++s) {
-            put(s + 1);  // (nobody reads stage s - 1 any more since the last barrier)
+            // (nobody reads stage s - 1 any more since the last barrier)
+            if ((s + 2) * BK > p.K) put(s + 1, true);
+            else put(s + 1, false);
             if (s + 2 < stages) fetch(s + 2);
             read(odd, s, 1);
             multiply(even);
@@ -544,27 +590,29 @@ hipError_t launch_matmul_int8(const Int8Params& p, int activation, int outDtype,
     return withType(outDtype, [&](auto element) {
         typedef decltype(element) T;
         const bool aligned = multipleOf(p.a, 16) && multipleOf(p.b, 16) && p.lda % 16 == 0 && p.ldb % 16 == 0 && p.K % 16 == 0;
-        auto few = [&](auto isAligned, auto tokens) {
+        using std::integral_constant;
+        auto few = [&](auto loads, auto tokens) {
             constexpr int MT = decltype(tokens)::value;
             const dim3 grid(unsigned((p.N + 15) / 16), unsigned((p.M + 16 * MT - 1) / (16 * MT)));
-            matmul_int8_few_kernel<T, decltype(isAligned)::value, MT><<<grid, 512, 0, s>>>(p, activation);
+            matmul_int8_few_kernel<T, decltype(loads)::value, MT><<<grid, 512, 0, s>>>(p, activation);
             return hipGetLastError();
         };
-        auto fewOf = [&](auto isAligned) {
-            if (p.M <= 16) return few(isAligned, std::integral_constant<int, 1>{});
-            if (p.M <= 32) return few(isAligned, std::integral_constant<int, 2>{});
-            return few(isAligned, std::integral_constant<int, 4>{});
+        auto fewOf = [&](auto loads) {
+            if (p.M <= 16) return few(loads, integral_constant<int, 1>{});
+            if (p.M <= 32) return few(loads, integral_constant<int, 2>{});
+            return few(loads, integral_constant<int, 4>{});
         };
-        if (p.M <= 64) return aligned ? fewOf(std::true_type{}) : fewOf(std::false_type{});
+        auto tiles = [&](int edge) { return ((p.M + edge - 1) / edge) * ((p.N + edge - 1) / edge); };
+        // (up to 64 tokens, unless there are channels enough for tiles on every CU: 33 x 16384 x 2047 34 us this way, 20 in tiles; 64 x 4096 x 4096 13 and 17)
+        if (p.M <= 16 || (p.M <= 64 && tiles(64) < 256)) return aligned ? fewOf(integral_constant<CodeLoads, kAligned>{}) : fewOf(integral_constant<CodeLoads, kWords>{});
         if (p.N <= 16) {
             const unsigned grid = unsigned((p.M + 255) / 256);
-            if (aligned) matmul_int8_narrow_kernel<T, true><<<grid, 256, 0, s>>>(p, activation);
-            else matmul_int8_narrow_kernel<T, false><<<grid, 256, 0, s>>>(p, activation);
+            if (aligned) matmul_int8_narrow_kernel<T, kAligned><<<grid, 256, 0, s>>>(p, activation);
+            else matmul_int8_narrow_kernel<T, kWords><<<grid, 256, 0, s>>>(p, activation);
             return hipGetLastError();
         }
         // The largest tile that still gives every CU one (edges of 256 only with k long enough to hide their beginning and end: one fits a CU). 8192 x 4096 x 4096: 145
         // us with 256, 199 with 128, 300 with 64; 262144 x 256 x 256: 46, 43, 61 us; 2048 x 1024 x 1024: 16, 10, 9 us.
-        auto tiles = [&](int edge) { return ((p.M + edge - 1) / edge) * ((p.N + edge - 1) / edge); };
         auto launch = [&](auto edge, auto wavesM, auto wavesN, auto ring) {
             constexpr int E = decltype(edge)::value, WM = decltype(wavesM)::value, WN = decltype(wavesN)::value, R = decltype(ring)::value;
             const int tilesM = int((p.M + E - 1) / E), tilesN = (p.N + E - 1) / E;
@@ -572,7 +620,6 @@ hipError_t launch_matmul_int8(const Int8Params& p, int activation, int outDtype,
             else matmul_int8_tile_kernel<T, E, E, WM, WN, 2, false><<<unsigned(tiles(E)), 64 * WM * WN, 0, s>>>(p, activation, tilesM, tilesN);
             return hipGetLastError();
         };
-        using std::integral_constant;
         if (tiles(256) >= 256 && p.K >= 1024) return launch(integral_constant<int, 256>{}, integral_constant<int, 4>{}, integral_constant<int, 4>{}, integral_constant<int, 3>{});
         if (tiles(128) >= 256) return launch(integral_constant<int, 128>{}, integral_constant<int, 2>{}, integral_constant<int, 2>{}, integral_constant<int, 3>{});
         return launch(integral_constant<int, 64>{}, integral_constant<int, 2>{}, integral_constant<int, 1>{}, integral_constant<int, 4>{});
