@@ -142,6 +142,67 @@ __device__ __forceinline__ void withGates(const ScanParams& p, const T (&raw)[L]
     }
 }
 
+// The state behind spans 0 .. count - 1 of a call that is cut into them, from their (A, U) (of span 0 U is the state, whatever its A): the waves fold a part each and join.
+// One after the other the folds of 127 spans took 20 us, which is most of what a span's steps take.
+template <int NW, int V, int GV>
+__device__ __forceinline__ void foldBefore(const float* wa, const float* wu, long long stride, int count, int w, int lane, float (&joined)[NW][GV + V][64], float (&h)[V]) {
+    const int each = (count + NW - 1) / NW, last = min(count, (w + 1) * each);
+    float A[GV], U[V];
+#pragma unroll
+    for (int v = 0; v < GV; ++v) A[v] = 1.f;
+#pragma unroll
+    for (int v = 0; v < V; ++v) U[v] = 0.f;
+#pragma unroll 4
+    for (int s = w * each; s < last; ++s) {
+        float a[GV];
+#pragma unroll
+        for (int v = 0; v < GV; ++v) {
+            a[v] = s == 0 ? 0.f : wa[s * stride + v];
+            A[v] *= a[v];
+        }
+#pragma unroll
+        for (int v = 0; v < V; ++v) U[v] = fmaf(a[GV == V ? v : 0], U[v], wu[s * stride + v]);
+    }
+#pragma unroll
+    for (int v = 0; v < GV; ++v) joined[w][v][lane] = A[v];
+#pragma unroll
+    for (int v = 0; v < V; ++v) joined[w][GV + v][lane] = U[v];
+    __syncthreads();
+#pragma unroll
+    for (int v = 0; v < V; ++v) h[v] = 0.f;
+#pragma unroll 2
+    for (int j = 0; j < NW; ++j)
+#pragma unroll
+        for (int v = 0; v < V; ++v) h[v] = fmaf(joined[j][GV == V ? v : 0][lane], h[v], joined[j][GV + v][lane]);
+}
+
+// What spans first .. count - 1 pass back of the gradient k that enters them from behind, from their (A, D)
+template <int NW, int V, int GV>
+__device__ __forceinline__ void foldBehind(const float* wa, const float* wd, long long stride, int first, int count, int w, int lane, float (&joined)[NW][GV + V][64], float (&k)[V]) {
+    const int each = (max(0, count - first) + NW - 1) / NW, from = min(count, first + w * each), last = min(count, from + each);
+    float A[GV], D[V];
+#pragma unroll
+    for (int v = 0; v < GV; ++v) A[v] = 1.f;
+#pragma unroll
+    for (int v = 0; v < V; ++v) D[v] = 0.f;
+#pragma unroll 4
+    for (int s = from; s < last; ++s) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) D[v] = fmaf(A[GV == V ? v : 0], wd[s * stride + v], D[v]);
+#pragma unroll
+        for (int v = 0; v < GV; ++v) A[v] *= wa[s * stride + v];
+    }
+#pragma unroll
+    for (int v = 0; v < GV; ++v) joined[w][v][lane] = A[v];
+#pragma unroll
+    for (int v = 0; v < V; ++v) joined[w][GV + v][lane] = D[v];
+    __syncthreads();
+#pragma unroll 2
+    for (int j = NW - 1; j >= 0; --j)
+#pragma unroll
+        for (int v = 0; v < V; ++v) k[v] = fmaf(joined[j][GV == V ? v : 0][lane], k[v], joined[j][GV + v][lane]);
+}
+
 // Forward.  AGGREGATE: only (A, U) of this workgroup's span, span 0 with h0 folded in (its A slot then holds h0 for the second launch: d_last may be d_h0).  The second
 // launch takes the spans from the last to the first: what the first launch read last is what the memory-side cache still holds.
 template <class T, int NW, int V, bool SHARED, bool AGGREGATE>
@@ -174,23 +235,20 @@ __global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW) void scan_channels_kernel(
                 for (int v = 0; v < V; ++v) p.ws[stored + v] = h[v];
         }
     }
-    if (!AGGREGATE && plan.chunks > 1) {
-        const float* const wa = p.ws + stored;
-        const float* const wu = wa + plane;
-        if (span == 0) {
-#pragma unroll
-            for (int v = 0; v < V; ++v) h[v] = wa[v];
-        } else {
-#pragma unroll
-            for (int v = 0; v < V; ++v) h[v] = wu[v];
-#pragma unroll 4
-            for (int s = 1; s < span; ++s)
-#pragma unroll
-                for (int v = 0; v < V; ++v) h[v] = fmaf(wa[(long long)s * p.C + v], h[v], wu[(long long)s * p.C + v]);
-        }
-    }
     __shared__ float joined[NW == 1 ? 1 : 2][NW][GV + V][NW == 1 ? 1 : 64];
     int buffer = 0;
+    if constexpr (NW > 1 && !AGGREGATE) {
+        if (plan.chunks > 1) {
+            const float* const wa = p.ws + stored;
+            if (span == 0) {
+#pragma unroll
+                for (int v = 0; v < V; ++v) h[v] = wa[v];
+            } else {
+                foldBefore<NW, V, GV>(wa, wa + plane, p.C, span, w, lane, joined[0], h);
+                buffer = 1;
+            }
+        }
+    }
     for (int tile = begin; tile < end; tile += NW * L) {
         const int i0 = tile + w * L;
         T rawG[L][GV], rawX[L][V];
@@ -406,23 +464,18 @@ __global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW, 4) void scan_channels_back
         h[v] = p.h0 ? p.h0[state + v] : 0.f;
         k[v] = p.dlast ? p.dlast[state + v] : 0.f;
     }
-    if (plan.chunks > 1) {
-        const float* const wa = ws.spans + (b * plan.chunks) * p.C + ch.c;
-        if (span > 0) {
-#pragma unroll
-            for (int v = 0; v < V; ++v) h[v] = wa[ws.plane + v];
-#pragma unroll 4
-            for (int s = 1; s < span; ++s)
-#pragma unroll
-                for (int v = 0; v < V; ++v) h[v] = fmaf(wa[(long long)s * p.C + v], h[v], wa[ws.plane + (long long)s * p.C + v]);
-        }
-#pragma unroll 4
-        for (int s = plan.chunks - 1; s > span; --s)
-#pragma unroll
-            for (int v = 0; v < V; ++v) k[v] = fmaf(wa[(long long)s * p.C + v], k[v], wa[2 * ws.plane + (long long)s * p.C + v]);
-    }
     __shared__ float joined[NW == 1 ? 1 : 2][NW][GV + 3 * V][NW == 1 ? 1 : 64];
     int buffer = 0;
+    if constexpr (NW > 1) {
+        if (plan.chunks > 1) {
+            typedef float Fold[NW][GV + V][64];
+            static_assert(sizeof(Fold) <= sizeof(joined[0]), "a fold borrows a buffer");
+            const float* const wa = ws.spans + (b * plan.chunks) * p.C + ch.c;
+            if (span > 0) foldBefore<NW, V, GV>(wa, wa + ws.plane, p.C, span, w, lane, reinterpret_cast<Fold&>(joined[0]), h);
+            foldBehind<NW, V, GV>(wa, wa + 2 * ws.plane, p.C, span + 1, plan.chunks, w, lane, reinterpret_cast<Fold&>(joined[1]), k);
+            __syncthreads();  // (the walk below begins with the first buffer, and a wave may still be reading the second one)
+        }
+    }
     if (kept && plan.chunks == 1) {
         // one span: the states at the head of every tile, for the walk back
         float at[V];
@@ -1117,8 +1170,9 @@ ScanPlan planScan(const ScanParams& p, int dtype, bool backward) {
     plan.slots = plan.parts = plan.vec = plan.chunks = plan.waves = 1;
     const long long step = std::llabs(p.xs[1]), next = std::llabs(p.xs[2]) * p.G;
     // Lanes along the steps where steps lie closer together than gates (colours along a ray: step 4, next ray's far away), or where there are too few
-    // gates beside each other to fill half a wave.
-    plan.rows = p.G <= 4 && (p.Cg < 32 || step < next);
+    // gates beside each other: 64 x 4096 steps of 6 channels take 31 us with lanes along the steps and 27 along the channels, backward 54 and 55; 4 channels
+    // 19 and 27, 28 and 53; 12 channels 56 and 28, 115 and 58.
+    plan.rows = p.G <= 4 && (p.Cg < 10 || step < next);
     if (plan.rows) {
         const int K = rowSteps(p.T, backward);
         plan.width = std::min(64, powerOfTwoAtLeast((p.T + K - 1) / K));

@@ -17,7 +17,7 @@ struct Range {
     bool operator&&(const Range& o) const { return first < o.last && o.first < last; }
 };
 
-// 0: the addresses of the operand leave 64 bits (or its sizes do)
+// false: the operand's addresses leave 64 bits, or it does not begin at a multiple of its element
 bool rangeOf(const char* name, const void* ptr, size_t element, int dims, const long long* size, const long long* stride, Range& r) {
     r.name = name;
     if (!ptr) return true;
@@ -29,7 +29,7 @@ bool rangeOf(const char* name, const void* ptr, size_t element, int dims, const 
     }
     const __int128 base = reinterpret_cast<unsigned long long>(ptr);
     const __int128 first = base + lo * __int128(element), last = base + (hi + 1) * __int128(element);
-    if (first < 0 || last > (__int128(1) << 63)) return false;
+    if (first < 0 || last > (__int128(1) << 63) || base % __int128(element) != 0) return false;
     r.first = (unsigned long long)first;
     r.last = (unsigned long long)last;
     return true;
@@ -152,12 +152,12 @@ int fvsrn_gated_scan(const fvsrn_scan_desc* desc, const void* d_gate, const void
         const size_t need = c.plan.wsFloats * sizeof(float);
         if (need > workspace_bytes || (need && !d_workspace))
             return fail(FVSRN_ERR_INVALID_ARGUMENT, "workspace too small: " + std::to_string(need) + " bytes are needed (fvsrn_gated_scan_workspace)");
-        const long long wsSize[1] = {(long long)need};
+        const long long wsSize[1] = {(long long)c.plan.wsFloats};
         Range gate, x, h0, len, out, last, ws;
         if (!rangeOf("gate", d_gate, e, 3, gates, p.gs, gate) || !rangeOf("x", d_x, e, 3, full, p.xs, x) || !rangeOf("h0", d_h0, 4, 2, ends, endStride, h0) ||
             !rangeOf("lengths", d_lengths, 4, 1, ends, one, len) || !rangeOf("out", d_out, e, 3, full, p.os, out) ||
-            !rangeOf("last", d_last, 4, 2, ends, endStride, last) || !rangeOf("the workspace", need ? d_workspace : nullptr, 1, 1, wsSize, one, ws))
-            return fail(FVSRN_ERR_INVALID_ARGUMENT, "an operand reaches beyond the address space");
+            !rangeOf("last", d_last, 4, 2, ends, endStride, last) || !rangeOf("the workspace", need ? d_workspace : nullptr, 4, 1, wsSize, one, ws))
+            return fail(FVSRN_ERR_INVALID_ARGUMENT, "an operand is not aligned to its elements or reaches beyond the address space");
         std::string clash = overlapping({out, last, ws}, {gate, x, len});
         if (clash.empty()) clash = overlapping({out, ws}, {h0, last});
         if (clash.empty()) clash = overlapping({out}, {ws});
@@ -190,14 +190,14 @@ int fvsrn_gated_scan_backward(const fvsrn_scan_desc* desc, const void* d_gate, c
         const size_t need = c.plan.wsFloats * sizeof(float);
         if (need > workspace_bytes || (need && !d_workspace))
             return fail(FVSRN_ERR_INVALID_ARGUMENT, "workspace too small: " + std::to_string(need) + " bytes are needed (fvsrn_gated_scan_workspace)");
-        const long long wsSize[1] = {(long long)need};
+        const long long wsSize[1] = {(long long)c.plan.wsFloats};
         Range gate, x, h0, len, dout, dlast, dgate, dx, dh0, ws;
         if (!rangeOf("gate", d_gate, e, 3, gates, p.gs, gate) || !rangeOf("x", d_x, e, 3, full, p.xs, x) || !rangeOf("h0", d_h0, 4, 2, ends, endStride, h0) ||
             !rangeOf("lengths", d_lengths, 4, 1, ends, one, len) || !rangeOf("dout", d_dout, e, 3, full, p.ds, dout) ||
             !rangeOf("dlast", d_dlast, 4, 2, ends, endStride, dlast) || !rangeOf("dgate", d_dgate, e, 3, gates, p.dgs, dgate) ||
             !rangeOf("dx", d_dx, e, 3, full, p.dxs, dx) || !rangeOf("dh0", d_dh0, 4, 2, ends, endStride, dh0) ||
-            !rangeOf("the workspace", need ? d_workspace : nullptr, 1, 1, wsSize, one, ws))
-            return fail(FVSRN_ERR_INVALID_ARGUMENT, "an operand reaches beyond the address space");
+            !rangeOf("the workspace", need ? d_workspace : nullptr, 4, 1, wsSize, one, ws))
+            return fail(FVSRN_ERR_INVALID_ARGUMENT, "an operand is not aligned to its elements or reaches beyond the address space");
         std::string clash = overlapping({dgate, dx, dh0, ws}, {gate, x, h0, len, dout, dlast});
         if (clash.empty()) clash = overlapping({dgate, dx, ws}, {dh0});
         if (clash.empty()) clash = overlapping({dgate, dx}, {ws});
@@ -227,7 +227,7 @@ int fvsrn_quantize_rows(const void* d_x, int dtype, long long rows, int cols, lo
         const long long size[2] = {rows, cols}, sx[2] = {ldx, 1}, sc[2] = {ldc, 1}, one[1] = {1};
         Range x, codes, scales;
         if (!rangeOf("x", d_x, elementSize(dtype), 2, size, sx, x) || !rangeOf("the codes", d_codes, 1, 2, size, sc, codes) || !rangeOf("the scales", d_scales, 4, 1, size, one, scales))
-            return fail(FVSRN_ERR_INVALID_ARGUMENT, "an operand reaches beyond the address space");
+            return fail(FVSRN_ERR_INVALID_ARGUMENT, "an operand is not aligned to its elements or reaches beyond the address space");
         std::string clash = overlapping({codes, scales}, {x});
         if (clash.empty()) clash = overlapping({codes}, {scales});
         if (!clash.empty()) return fail(FVSRN_ERR_INVALID_ARGUMENT, clash);
@@ -257,7 +257,7 @@ int fvsrn_matmul_int8(const signed char* d_a, long long lda, const float* d_scal
         Range a, b, out, scaleA, scaleB, bias;
         if (!rangeOf("a", d_a, 1, 2, as, sa, a) || !rangeOf("b", d_b, 1, 2, bs, sb, b) || !rangeOf("out", d_out, elementSize(out_dtype), 2, os, so, out) ||
             !rangeOf("scale_a", d_scale_a, 4, 1, as, one, scaleA) || !rangeOf("scale_b", d_scale_b, 4, 1, bs, one, scaleB) || !rangeOf("bias", d_bias, 4, 1, bs, one, bias))
-            return fail(FVSRN_ERR_INVALID_ARGUMENT, "an operand reaches beyond the address space");
+            return fail(FVSRN_ERR_INVALID_ARGUMENT, "an operand is not aligned to its elements or reaches beyond the address space");
         const std::string clash = overlapping({out}, {a, b, scaleA, scaleB, bias});
         if (!clash.empty()) return fail(FVSRN_ERR_INVALID_ARGUMENT, clash);
         if (fvsrn_device_count() == 0) return noDevice();

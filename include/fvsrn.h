@@ -488,8 +488,8 @@ int fvsrn_render_volume(fvsrn_scene* scene, fvsrn_volume* volume, int source, in
  * gradients.  No reference counterpart.
  *
  * Conventions on top of those at the head of this file: all pointers are device pointers of the current device; strides and sizes are in
- * elements; the calls allocate nothing (where one needs scratch memory the caller hands it in), read no device memory on the host and may
- * be captured into a graph.  Outputs must not overlap inputs or each other (FVSRN_ERR_INVALID_ARGUMENT where their address ranges do),
+ * elements, operands begin at a multiple of their element; the calls allocate nothing (where one needs scratch memory the caller hands it in, for
+ * this call alone until it is done), read no device memory on the host and may be captured into a graph.  Outputs must not overlap inputs or each other (FVSRN_ERR_INVALID_ARGUMENT where their address ranges do),
  * except where an entry says so.  A size of zero is a call that does nothing more than its definition says (no rows: nothing). */
 typedef enum { FVSRN_TENSOR_F32 = 0, FVSRN_TENSOR_F16 = 1, FVSRN_TENSOR_BF16 = 2 } fvsrn_tensor_dtype;
 

@@ -451,7 +451,9 @@ def plain_product(a, sa, b, sb, bias, activation, param, dtype):
 
 
 PRODUCTS = [(1, 1, 1), (1, 17, 5), (3, 64, 64), (65, 63, 130), (130, 257, 100), (64, 64, 16), (257, 129, 1000), (1, 100, 4096), (16, 300, 777), (17, 48, 1024), (33, 33, 33),
-            (128, 256, 128), (300, 300, 320), (1000, 4, 250), (513, 520, 512), (5, 1, 131071), (600, 1, 64), (1, 3001, 70), (260, 256, 256), (2048, 192, 96)]
+            (128, 256, 128), (300, 300, 320), (1000, 4, 250), (513, 520, 512), (5, 1, 131071), (600, 1, 64), (1, 3001, 70), (260, 256, 256), (2048, 192, 96),
+            (300, 40, 7), (100, 16, 15), (300, 300, 1), (70, 100, 31), (300, 20, 17), (5000, 16, 250), (40, 20000, 33), (20, 20000, 64), (300, 70, 48), (3000, 2900, 80),
+            (4200, 4100, 1040), (4200, 4100, 1031)]
 
 
 @pytest.mark.gpu
@@ -498,6 +500,68 @@ def test_product_strides_and_neighbours():
         assert torch.equal(capi.matmul_int8(one_row, one[:M], b, one[:N]).cpu(), want[:1].expand(M, N))
     e = torch.empty(0, 64, dtype=torch.int8, device="cuda")
     assert capi.matmul_int8(e, torch.empty(0, device="cuda"), b[:, :64], one[:b.shape[0]]).shape == (0, b.shape[0])
+
+
+@pytest.mark.gpu
+def test_operands_beyond_32_bits_of_offset():
+    """Rows and sequences more than 2^31 elements apart, and more than 2^32 bytes."""
+    far = 2 ** 31 + 2 ** 20
+    g = torch.Generator().manual_seed(8)
+    a = torch.empty(2 * far + 64, dtype=torch.int8, device="cuda").as_strided((3, 64), (far, 1))
+    a.copy_(torch.randint(-128, 128, (3, 64), generator=g, dtype=torch.int8))
+    b = torch.randint(-128, 128, (100, 64), generator=g, dtype=torch.int8).cuda()
+    one = torch.ones(100, device="cuda")
+    out = torch.empty(2 * far + 100, dtype=F16, device="cuda").as_strided((3, 100), (far, 1))
+    want = (a.cpu().long() @ b.cpu().long().t()).float()
+    assert torch.equal(capi.matmul_int8(a, one[:3], b, one).cpu(), want)
+    capi.matmul_int8(a, one[:3] / 1024, b, one, out=out)
+    assert torch.equal(out.cpu(), (want / 1024).to(F16))
+    many = a[:1].expand(300, 64)
+    assert torch.equal(capi.matmul_int8(a[2:].expand(300, 64), one[:1].expand(300).contiguous(), b, one).cpu(), want[2:].expand(300, 100)) and many.stride(0) == 0
+    x = torch.empty(2 * far + 5000, dtype=F16, device="cuda").as_strided((3, 64), (far, 1))
+    x.copy_(torch.randn(3, 64, generator=g))
+    assert_codes(x, *capi.quantize_rows(x, codes=torch.empty(2 * far + 64, dtype=torch.int8, device="cuda").as_strided((3, 64), (far, 1))))
+    how = modes(7)
+    for shape in ((2, 6, 3, 1), (2, 300, 64, 64)):
+        B, T, Ch, Cg = shape
+        x = torch.empty(far + T * Ch, dtype=F16, device="cuda").as_strided((B, T, Ch), (far, Ch, 1))
+        x.copy_(torch.randn(B, T, Ch, generator=g))
+        gate, d = torch.rand(B, T, Cg, generator=g).to(F16).cuda(), torch.randn(B, T, Ch, generator=g).to(F16).cuda()
+        want = plain_scan(gate, x, d, None, **how)
+        out, last = capi.gated_scan(gate, x, out=torch.empty(far + T * Ch, dtype=F16, device="cuda").as_strided((B, T, Ch), (far, Ch, 1)), **how)
+        dgate, dx, _ = capi.gated_scan_backward(gate, x, d, dx=torch.empty(far + T * Ch, dtype=F16, device="cuda").as_strided((B, T, Ch), (far, Ch, 1)), **how)
+        for name, got in (("out", out), ("last", last), ("dgate", dgate), ("dx", dx)):
+            assert_within(got, want[name], name)
+    # steps that far apart
+    x = torch.empty(4 * far + 64, dtype=F16, device="cuda").as_strided((1, 5, 64), (1, far, 1))
+    x.copy_(torch.randn(1, 5, 64, generator=g))
+    gate = torch.rand(1, 5, 64, generator=g).to(F16).cuda()
+    assert_within(capi.gated_scan(gate, x, **how)[0], plain_scan(gate, x, **how)["out"], "out")
+
+
+@pytest.mark.gpu
+def test_scan_negative_strides():
+    """The C ABI takes strides that run backwards (an array seen from its end): the same as the turned tensor."""
+    for B, T, Ch, Cg in ((3, 40, 3, 1), (2, 700, 64, 64), (2, 50, 96, 12)):
+        how = modes(3)
+        case = scan_inputs(B, T, Ch, Cg, F32, how["gate_mode"], 3)
+        turned = {k: case[k].flip(1) for k in ("gate", "x", "dout")}
+        want = plain_scan(turned["gate"], turned["x"], turned["dout"], case["dlast"], h0=case["h0"], **how)
+        d = desc(B, T, Ch, Cg, gate_mode=how["gate_mode"], input_mode=how["input_mode"], gate_scale=how["gate_scale"], x_stride=(T * Ch, -Ch, 1), gate_stride=(T * Cg, -Cg, 1),
+                 dout_stride=(T * Ch, -Ch, 1), out_stride=(T * Ch, -Ch, 1), dx_stride=(T * Ch, -Ch, 1), dgate_stride=(T * Cg, -Cg, 1))
+        n = [C.c_size_t(0), C.c_size_t(0)]
+        for backward in (0, 1):
+            assert capi.lib().fvsrn_gated_scan_workspace(C.byref(d), backward, C.byref(n[backward])) == 0
+        ws = torch.empty(max(n[0].value, n[1].value, 4), dtype=torch.uint8, device="cuda")
+        out, last = torch.empty(B, T, Ch, device="cuda"), torch.empty(B, Ch, device="cuda")
+        dgate, dx, dh0 = torch.empty(B, T, Cg, device="cuda"), torch.empty(B, T, Ch, device="cuda"), torch.empty(B, Ch, device="cuda")
+        end = lambda t: t[:, -1:].data_ptr()  # noqa: E731
+        s = torch.cuda.current_stream().cuda_stream
+        assert capi.lib().fvsrn_gated_scan(C.byref(d), end(case["gate"]), end(case["x"]), case["h0"].data_ptr(), None, end(out), last.data_ptr(), ws.data_ptr(), n[0], s) == 0
+        assert capi.lib().fvsrn_gated_scan_backward(C.byref(d), end(case["gate"]), end(case["x"]), case["h0"].data_ptr(), None, end(case["dout"]), case["dlast"].data_ptr(), end(dgate),
+                                                    end(dx), dh0.data_ptr(), ws.data_ptr(), n[1], s) == 0
+        for name, got in (("out", out.flip(1)), ("last", last), ("dgate", dgate.flip(1)), ("dx", dx.flip(1)), ("dh0", dh0)):
+            assert_within(got, want[name], name)
 
 
 @pytest.mark.gpu
@@ -621,6 +685,10 @@ def test_scan_refusals():
     assert scan_call(desc(x_stride=(0, 0, 0), gate_stride=(0, 0, 0))) == OK
     assert scan_call(desc(x_stride=(30, -6, 1))) == OK
     assert scan_call(desc(x_stride=(1 << 62, 6, 1))) == -1
+    # operands begin at an element
+    for name in ("gate", "x", "h0", "out", "last"):
+        assert scan_call(desc(), **{name: 10 * GIB + 2}) == -1, name
+    assert scan_call(desc(dtype=1), x=10 * GIB + 2) == OK and scan_call(desc(dtype=1), x=10 * GIB + 1) == -1 and scan_call(desc(), lengths=10 * GIB + 2) == -1
     assert scan_call(desc(B=1 << 20, T=1 << 20, Ch=1024, Cg=1024)) == -4
 
 
@@ -666,7 +734,8 @@ def test_product_and_codes_refusals():
 
     assert product() == OK and product(bias=None) == OK and product(a=GIB + 1, lda=67) == OK
     for bad in (dict(dtype=3), dict(act=6), dict(act=-1), dict(act=1, p=0.0), dict(act=2, p=math.inf), dict(act=3, p=math.nan), dict(M=-1), dict(N=-1), dict(K=0), dict(lda=63), dict(ldb=63),
-                dict(ldo=15), dict(a=None), dict(b=None), dict(sa=None), dict(sb=None), dict(out=None), dict(out=GIB + 63), dict(out=3 * GIB), dict(out=2 * GIB), dict(out=5 * GIB)):
+                dict(ldo=15), dict(a=None), dict(b=None), dict(sa=None), dict(sb=None), dict(out=None), dict(out=GIB + 63), dict(out=3 * GIB), dict(out=2 * GIB), dict(out=5 * GIB),
+                dict(sa=2 * GIB + 2), dict(sb=4 * GIB + 1), dict(bias=5 * GIB + 3), dict(out=6 * GIB + 2)):
         assert product(**bad) == -1, bad
     assert product(K=131072, lda=131072, ldb=131072) == -4 and product(K=131071, lda=131071, ldb=131071) == OK
     assert product(M=0, a=None, out=None) == 0 and product(N=0) == 0
