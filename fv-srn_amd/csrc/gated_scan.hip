@@ -45,6 +45,12 @@ __device__ __forceinline__ void gateOf(float g, float scale, float& a, float& re
     }
 }
 
+// A barrier for what goes through LDS: __syncthreads would also wait for the stores of the last tile and the loads of the next one.
+__device__ __forceinline__ void ldsBarrier() {
+    __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+    asm volatile("s_barrier" ::: "memory");
+}
+
 __device__ __forceinline__ int lengthOf(const ScanParams& p, long long b) {
     return p.lengths ? min(max(p.lengths[b], 0), p.T) : p.T;
 }
@@ -102,18 +108,23 @@ inline long long channelBlocks(const ScanParams& p, const ScanPlan& plan) {
 // V channels of steps i .. i + L - 1, zeros from step `end` on
 template <class T, int V, int L>
 __device__ __forceinline__ void loadChannels(const T* p, long long step, int i, int n, int end, int reverse, T (&to)[L][V]) {
-    if (i + L <= end) {  // (the same for all lanes)
+    if (i >= end) {  // (these conditions are the same for all lanes)
+#pragma unroll
+        for (int k = 0; k < L; ++k)
+#pragma unroll
+            for (int v = 0; v < V; ++v) to[k][v] = T(0.f);
+    } else if (i + L <= end) {
         const T* at = p + positionOf(i, n, reverse) * step;
         const long long next = reverse ? -step : step;
 #pragma unroll
         for (int k = 0; k < L; ++k) loadWide<T, V>(to[k], at + k * next);
-    } else {
+    } else {  // every load is made, the last step's again for those behind it: a branch for each would have them wait for each other
 #pragma unroll
-        for (int k = 0; k < L; ++k) {
+        for (int k = 0; k < L; ++k) loadWide<T, V>(to[k], p + positionOf(min(i + k, end - 1), n, reverse) * step);
 #pragma unroll
-            for (int v = 0; v < V; ++v) to[k][v] = T(0.f);
-            if (i + k < end) loadWide<T, V>(to[k], p + positionOf(i + k, n, reverse) * step);
-        }
+        for (int k = 0; k < L; ++k)
+#pragma unroll
+            for (int v = 0; v < V; ++v) to[k][v] = i + k < end ? to[k][v] : T(0.f);
     }
 }
 
@@ -167,7 +178,7 @@ __device__ __forceinline__ void foldBefore(const float* wa, const float* wu, lon
     for (int v = 0; v < GV; ++v) joined[w][v][lane] = A[v];
 #pragma unroll
     for (int v = 0; v < V; ++v) joined[w][GV + v][lane] = U[v];
-    __syncthreads();
+    ldsBarrier();
 #pragma unroll
     for (int v = 0; v < V; ++v) h[v] = 0.f;
 #pragma unroll 2
@@ -196,7 +207,7 @@ __device__ __forceinline__ void foldBehind(const float* wa, const float* wd, lon
     for (int v = 0; v < GV; ++v) joined[w][v][lane] = A[v];
 #pragma unroll
     for (int v = 0; v < V; ++v) joined[w][GV + v][lane] = D[v];
-    __syncthreads();
+    ldsBarrier();
 #pragma unroll 2
     for (int j = NW - 1; j >= 0; --j)
 #pragma unroll
@@ -249,11 +260,14 @@ __global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW) void scan_channels_kernel(
             }
         }
     }
+    T rawG[L][GV], rawX[L][V];
+    auto load = [&](int i) {
+        loadChannels<T, GV, L>(gp, p.gs[1], i, n, inside, p.reverse, rawG);
+        loadChannels<T, V, L>(xp, p.xs[1], i, n, inside, p.reverse, rawX);
+    };
+    load(begin + w * L);
     for (int tile = begin; tile < end; tile += NW * L) {
         const int i0 = tile + w * L;
-        T rawG[L][GV], rawX[L][V];
-        loadChannels<T, GV, L>(gp, p.gs[1], i0, n, inside, p.reverse, rawG);
-        loadChannels<T, V, L>(xp, p.xs[1], i0, n, inside, p.reverse, rawX);
         float a[L][GV], u[L][V], a2[GV], u2[V];
 #pragma unroll
         for (int v = 0; v < V; ++v) u2[v] = 0.f;
@@ -268,6 +282,7 @@ __global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW) void scan_channels_kernel(
                 u2[c] = fmaf(gate, u2[c], u[k][c]);
             }
         });
+        if (tile + NW * L < end) load(i0 + NW * L);  // (on its way while this tile is joined and stored)
         float pre[V];
 #pragma unroll
         for (int v = 0; v < V; ++v) pre[v] = h[v];
@@ -276,7 +291,7 @@ __global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW) void scan_channels_kernel(
             for (int v = 0; v < GV; ++v) joined[buffer][w][v][lane] = a2[v];
 #pragma unroll
             for (int v = 0; v < V; ++v) joined[buffer][w][GV + v][lane] = u2[v];
-            __syncthreads();  // (one barrier a tile: the two buffers take turns, and a wave can only be one tile ahead)
+            ldsBarrier();  // (one barrier a tile: the two buffers take turns, and a wave can only be one tile ahead)
 #pragma unroll 2
             for (int j = 0; j < NW; ++j) {
                 float aj[GV];
@@ -377,6 +392,13 @@ __global__ __launch_bounds__(64 * NW) void scan_channels_spans_kernel(const Scan
     }
     __shared__ float joined[2][NW][GV + 2 * V][64];
     int buffer = 0;
+    T rawG[L][GV], rawX[L][V], rawD[L][V];
+    auto load = [&](int i) {
+        loadChannels<T, GV, L>(gp, p.gs[1], i, n, end, p.reverse, rawG);
+        loadChannels<T, V, L>(xp, p.xs[1], i, n, end, p.reverse, rawX);
+        if (dp) loadChannels<T, V, L>(dp, p.ds[1], i, n, end, p.reverse, rawD);
+    };
+    load(begin + w * L);
     for (int tile = begin, j = 0; tile < end; tile += NW * L, ++j) {
         if (tilesOfSpan > 1 && w == 0 && ch.live) {
 #pragma unroll
@@ -386,10 +408,6 @@ __global__ __launch_bounds__(64 * NW) void scan_channels_spans_kernel(const Scan
             }
         }
         const int i0 = tile + w * L;
-        T rawG[L][GV], rawX[L][V], rawD[L][V];
-        loadChannels<T, GV, L>(gp, p.gs[1], i0, n, end, p.reverse, rawG);
-        loadChannels<T, V, L>(xp, p.xs[1], i0, n, end, p.reverse, rawX);
-        if (dp) loadChannels<T, V, L>(dp, p.ds[1], i0, n, end, p.reverse, rawD);
         float a2[GV], u2[V], d2[V];
 #pragma unroll
         for (int v = 0; v < V; ++v) u2[v] = d2[v] = 0.f;
@@ -403,6 +421,7 @@ __global__ __launch_bounds__(64 * NW) void scan_channels_spans_kernel(const Scan
                 if (dp) d2[c] = fmaf(a2[v], toFloat(rawD[k][c]), d2[c]);
             }
         });
+        if (tile + NW * L < end) load(i0 + NW * L);
 #pragma unroll
         for (int v = 0; v < GV; ++v) joined[buffer][w][v][lane] = a2[v];
 #pragma unroll
@@ -410,7 +429,7 @@ __global__ __launch_bounds__(64 * NW) void scan_channels_spans_kernel(const Scan
             joined[buffer][w][GV + v][lane] = u2[v];
             joined[buffer][w][GV + V + v][lane] = d2[v];
         }
-        __syncthreads();
+        ldsBarrier();
 #pragma unroll 2
         for (int s = 0; s < NW; ++s) {
             float as[GV];
@@ -473,7 +492,7 @@ __global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW, 4) void scan_channels_back
             const float* const wa = ws.spans + (b * plan.chunks) * p.C + ch.c;
             if (span > 0) foldBefore<NW, V, GV>(wa, wa + ws.plane, p.C, span, w, lane, reinterpret_cast<Fold&>(joined[0]), h);
             foldBehind<NW, V, GV>(wa, wa + 2 * ws.plane, p.C, span + 1, plan.chunks, w, lane, reinterpret_cast<Fold&>(joined[1]), k);
-            __syncthreads();  // (the walk below begins with the first buffer, and a wave may still be reading the second one)
+            ldsBarrier();  // (the walk below begins with the first buffer, and a wave may still be reading the second one)
         }
     }
     if (kept && plan.chunks == 1) {
@@ -504,7 +523,7 @@ __global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW, 4) void scan_channels_back
                 for (int v = 0; v < GV; ++v) joined[buffer][w][v][lane] = a2[v];
 #pragma unroll
                 for (int v = 0; v < V; ++v) joined[buffer][w][GV + v][lane] = u2[v];
-                __syncthreads();
+                ldsBarrier();
 #pragma unroll 2
                 for (int s = 0; s < NW; ++s)
 #pragma unroll
@@ -516,12 +535,15 @@ __global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW, 4) void scan_channels_back
             }
         }
     }
+    T rawG[L][GV], rawX[L][V], rawD[L][V];
+    auto load = [&](int i) {
+        loadChannels<T, GV, L>(gp, p.gs[1], i, n, inside, p.reverse, rawG);
+        loadChannels<T, V, L>(xp, p.xs[1], i, n, inside, p.reverse, rawX);
+        if (dp) loadChannels<T, V, L>(dp, p.ds[1], i, n, inside, p.reverse, rawD);
+    };
     for (int j = tiles - 1; j >= 0; --j) {
         const int i0 = begin + j * plan.tile + w * L;
-        T rawG[L][GV], rawX[L][V], rawD[L][V];
-        loadChannels<T, GV, L>(gp, p.gs[1], i0, n, inside, p.reverse, rawG);
-        loadChannels<T, V, L>(xp, p.xs[1], i0, n, inside, p.reverse, rawX);
-        if (dp) loadChannels<T, V, L>(dp, p.ds[1], i0, n, inside, p.reverse, rawD);
+        load(i0);
         // the state at the head of the tile: of a wave on its own its own, of waves that share one what wave 0 says below
         float head[V];
 #pragma unroll
@@ -569,7 +591,7 @@ __global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW, 4) void scan_channels_back
                 joined[buffer][w][GV + V + v][lane] = d2[v];
                 if (w == 0) joined[buffer][0][GV + 2 * V + v][lane] = head[v];
             }
-            __syncthreads();
+            ldsBarrier();
 #pragma unroll
             for (int v = 0; v < V; ++v) hw[v] = joined[buffer][0][GV + 2 * V + v][lane];
 #pragma unroll 2
@@ -593,45 +615,52 @@ __global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW, 4) void scan_channels_back
                 entry[q][v] = hw[v];
                 hw[v] = fmaf(a[q][SHARED ? 0 : v], hw[v], rest[q][SHARED ? 0 : v] * x[q][v]);
             }
+        // (what is needed of x and the states on the way in: the gate's gradient takes l times it)
+#pragma unroll
+        for (int q = 0; q < L; ++q)
+#pragma unroll
+            for (int v = 0; v < V; ++v) entry[q][v] = p.blend ? entry[q][v] - x[q][v] : entry[q][v];
+        float sum[L][GV];
 #pragma unroll
         for (int q = L - 1; q >= 0; --q) {
-            const int i = i0 + q;
-            const bool in = i < inside;
-            const long long t = positionOf(i, n, p.reverse);
-            T dx[V], dg[GV];
-            float sum = 0.f;
+#pragma unroll
+            for (int v = 0; v < GV; ++v) sum[q][v] = 0.f;
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                const float av = a[q][SHARED ? 0 : v], l = d[q][v] + kw[v];
-                dx[v] = fromFloat<T>(in ? rest[q][SHARED ? 0 : v] * l : 0.f);
-                float s = l * (p.blend ? entry[q][v] - x[q][v] : entry[q][v]);
-                if (SHARED) {
-                    sum += s;
-                } else {
-                    if (p.exp) s *= p.scale * av;
-                    if (V == 1) sum = s;
-                    else dg[v] = fromFloat<T>(in ? s : 0.f);
+                const int g = SHARED ? 0 : v;
+                const float l = d[q][v] + kw[v];
+                x[q][v] = rest[q][g] * l;  // the gradient of x
+                sum[q][g] = SHARED ? fmaf(l, entry[q][v], sum[q][g]) : l * entry[q][v];
+                kw[v] = a[q][g] * l;
+            }
+#pragma unroll
+            for (int v = 0; v < GV; ++v) sum[q][v] = p.exp ? sum[q][v] * (p.scale * a[q][v]) : sum[q][v];
+        }
+        const bool first = V > 1 || plan.slots == 1 || (lane & (plan.slots - 1)) == 0;
+        if (V == 1 && plan.slots > 1) {
+#pragma unroll
+            for (int q = 0; q < L; ++q) sum[q][0] = ch.live ? sum[q][0] : 0.f;
+            for (int o = 1; o < plan.slots; o <<= 1)
+#pragma unroll
+                for (int q = 0; q < L; ++q) sum[q][0] += __shfl_xor(sum[q][0], o, 64);
+        }
+        if (ch.live) {
+#pragma unroll
+            for (int q = 0; q < L; ++q) {
+                const int i = i0 + q;
+                if (i >= end) break;
+                const bool in = i < inside;
+                const long long t = positionOf(i, n, p.reverse);
+                T dx[V], dg[GV];
+#pragma unroll
+                for (int v = 0; v < V; ++v) dx[v] = fromFloat<T>(in ? x[q][v] : 0.f);
+#pragma unroll
+                for (int v = 0; v < GV; ++v) dg[v] = fromFloat<T>(in ? sum[q][v] : 0.f);
+                if (dxp) storeWide<T, V>(dxp + t * p.dxs[1], dx);
+                if (dgp && first) {
+                    if (V == 1 && plan.parts > 1) partial[t * (long long)p.Cg * plan.parts] = in ? sum[q][0] : 0.f;
+                    else storeWide<T, GV>(dgp + t * p.dgs[1], dg);
                 }
-                kw[v] = av * l;
-            }
-            if (SHARED) {
-                if (p.exp) sum *= p.scale * a[q][0];
-                dg[0] = fromFloat<T>(in ? sum : 0.f);
-            }
-            bool first = true;
-            if (V == 1) {
-                if (plan.slots > 1) {
-                    sum = ch.live ? sum : 0.f;
-                    for (int o = 1; o < plan.slots; o <<= 1) sum += __shfl_xor(sum, o, 64);
-                    first = (lane & (plan.slots - 1)) == 0;
-                }
-                dg[0] = fromFloat<T>(in ? sum : 0.f);
-            }
-            if (i >= end || !ch.live) continue;
-            if (dxp) storeWide<T, V>(dxp + t * p.dxs[1], dx);
-            if (dgp && first) {
-                if (V == 1 && plan.parts > 1) partial[t * (long long)p.Cg * plan.parts] = in ? sum : 0.f;
-                else storeWide<T, GV>(dgp + t * p.dgs[1], dg);
             }
         }
         if constexpr (NW == 1) {
@@ -1211,12 +1240,21 @@ ScanPlan planScan(const ScanParams& p, int dtype, bool backward) {
     plan.waves = units >= 4096 || p.T <= 2 * L ? 1 : kScanWaves;
     plan.tile = plan.waves * L;
     const int tiles = int((p.T + (long long)plan.tile - 1) / plan.tile);
-    // Spans: two workgroups for each CU, and at least two tiles a span.
+    // Spans: two workgroups for each CU (384 for the chip: 164 us where 512 take 138, 768 152, 2048 238), and at least two tiles a span.
     const long long want = plan.waves == 1 ? 1 : (512 + units - 1) / units;
     const int spans = int(std::max(1LL, std::min(want, (long long)tiles / 2)));
     const int tilesOfSpan = std::max(1, (tiles + spans - 1) / spans);
     plan.chunks = std::max(1, (tiles + tilesOfSpan - 1) / tilesOfSpan);
     plan.chunkSteps = tilesOfSpan * plan.tile;
+    // A few tiles of twice the waves in one launch are better than spans in two: 16 x 500 x 1024 23 us against 29, 100 x 1001 x 64 22 against 27, 1 x 256 x 256 10
+    // against 13; with few workgroups only up to two tiles (1 x 500 x 256: 18 us against 13).
+    const int wide = 2 * kScanWaves * L, wideTiles = int((p.T + (long long)wide - 1) / wide);
+    if (!backward && plan.chunks > 1 && wideTiles <= (units >= 96 ? 4 : 2)) {
+        plan.waves = 2 * kScanWaves;
+        plan.tile = wide;
+        plan.chunks = 1;
+        plan.chunkSteps = wideTiles * wide;
+    }
     plan.wsFloats = backward ? backwardFloats(p, plan) : plan.chunks > 1 ? 2 * size_t(p.B) * p.C * plan.chunks : 0;
     return plan;
 }
@@ -1246,6 +1284,10 @@ hipError_t launch_gated_scan(const ScanParams& p, const ScanPlan& plan, int dtyp
                 return hipGetLastError();
             }
             const dim3 grid(unsigned(units), unsigned(plan.chunks));
+            if (plan.waves > kScanWaves) {
+                scan_channels_kernel<T, 2 * kScanWaves, V, SHARED, false><<<grid, 128 * kScanWaves, 0, s>>>(p, plan, blocks, units);
+                return hipGetLastError();
+            }
             if (plan.chunks > 1) {
                 scan_channels_kernel<T, kScanWaves, V, SHARED, true><<<grid, 64 * kScanWaves, 0, s>>>(p, plan, blocks, units);
                 if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
