@@ -252,6 +252,7 @@ int fvsrn_matmul_int8(const signed char* d_a, long long lda, const float* d_scal
         if (!d_a || !d_b || !d_scale_a || !d_scale_b || !d_out) return fail(FVSRN_ERR_INVALID_ARGUMENT, "null pointer");
         if ((lda < K && !(lda == 0 || M == 1)) || (ldb < K && !(ldb == 0 || N == 1)) || (ldo < N && M > 1))
             return fail(FVSRN_ERR_INVALID_ARGUMENT, "a row stride is smaller than a row");
+        if (N > (1 << 26)) return fail(FVSRN_ERR_UNSUPPORTED, "too many channels for one launch, split the weights");
         if (M > (1LL << 31)) return fail(FVSRN_ERR_UNSUPPORTED, "too many rows for one launch, split the matrix");
         const long long as[2] = {M, K}, bs[2] = {N, K}, os[2] = {M, N}, sa[2] = {lda, 1}, sb[2] = {ldb, 1}, so[2] = {ldo, 1}, one[1] = {1};
         Range a, b, out, scaleA, scaleB, bias;

@@ -738,6 +738,7 @@ def test_product_and_codes_refusals():
                 dict(sa=2 * GIB + 2), dict(sb=4 * GIB + 1), dict(bias=5 * GIB + 3), dict(out=6 * GIB + 2)):
         assert product(**bad) == -1, bad
     assert product(K=131072, lda=131072, ldb=131072) == -4 and product(K=131071, lda=131071, ldb=131071) == OK
+    assert product(N=(1 << 26) + 1, ldo=1 << 27) == -4 and product(M=(1 << 31) + 1) == -4
     assert product(M=0, a=None, out=None) == 0 and product(N=0) == 0
     assert product(act=0, p=math.nan) == OK  # (ReLU has no parameter)
     assert product(lda=0) == OK and product(M=1, ldo=1, lda=1) == OK
