@@ -383,9 +383,10 @@ __global__ __launch_bounds__(256) void matmul_int8_narrow_kernel(const Int8Param
 // operands of a half are read while the half before is multiplied, so the matrix units have work queued at every wait.
 //   Not DIRECT (rows that are not aligned to 16 bytes): a stage goes through registers, asked for a stage ahead of its way into a ring of two -- unaligned addresses
 // are for registers only, and so is the masking of the chunk in which K ends.
-//   LDS holds rows of four 16-byte chunks, chunk c of row r at place c ^ swizzle(r), so that the 32 rows a wave reads at one k spread over all banks; the
-// loads write LDS in lane order, so it is their source that is permuted.  A wave's channels are paired -- column l of its piece j is channel 2 l + j -- so that a
-// lane stores two adjacent outputs and a wave whole 128-byte lines of 16-bit ones.
+//   LDS holds rows of four 16-byte chunks, chunk c of row r at place c ^ (r / 4) % 4, so that 16 rows read at one k lie in 64 different banks; the loads write LDS in
+// lane order, so it is their source that is permuted.  A wave's channels are paired -- column l of its piece j is channel 2 l + j -- so that a lane stores two adjacent
+// outputs and a wave whole 128-byte lines of 16-bit ones; they lie in LDS in the order in which they are read (every second row would meet every second
+// bank twice: half of the LDS cycles).
 template <class T, int TM, int TN, int WM, int WN, int RING, bool DIRECT>
 __global__ __launch_bounds__(64 * WM * WN) void matmul_int8_tile_kernel(const Int8Params p, const int activation, const int tilesM, const int tilesN) {
     constexpr int BK = 64, WAVES = WM * WN, PM = TM / WM / 32, STAGE = (TM + TN) * BK;
@@ -408,10 +409,11 @@ __global__ __launch_bounds__(64 * WM * WN) void matmul_int8_tile_kernel(const In
     int chunk[LOADS];
 #pragma unroll
     for (int j = 0; j < LOADS; ++j) {
-        const int row = (wave * LOADS + j) * 16 + (lane >> 2);  // of the tile: tokens, then channels
+        const int row = (wave * LOADS + j) * 16 + (lane >> 2);  // of the tile: tokens, then channels, of each 64 the even ones before the odd ones
         const bool token = row < TM;
-        chunk[j] = ((lane & 3) ^ ((token ? row >> 1 : row >> 2) & 3)) * 16;
-        source[j] = (token ? p.a + min(m0 + row, p.M - 1) * p.lda : p.b + (long long)min(n0 + row - TM, p.N - 1) * p.ldb) + (DIRECT ? chunk[j] : 0);
+        const int channel = ((row - TM) & ~63) + 2 * (row & 31) + ((row >> 5) & 1);
+        chunk[j] = ((lane & 3) ^ ((row >> 2) & 3)) * 16;
+        source[j] = (token ? p.a + min(m0 + row, p.M - 1) * p.lda : p.b + (long long)min(n0 + channel, p.N - 1) * p.ldb) + (DIRECT ? chunk[j] : 0);
     }
     const int stages = (p.K + BK - 1) / BK;
     Codes<kBytes> staged[LOADS];
@@ -441,11 +443,11 @@ __global__ __launch_bounds__(64 * WM * WN) void matmul_int8_tile_kernel(const In
 #pragma unroll
         for (int i = 0; i < PM; ++i) {
             const int row = wm + i * 32 + col;
-            o.a[i] = *reinterpret_cast<const int4_t*>(buffer + row * BK + (((kk * 2 + half) ^ ((row >> 1) & 3)) * 16));
+            o.a[i] = *reinterpret_cast<const int4_t*>(buffer + row * BK + (((kk * 2 + half) ^ ((row >> 2) & 3)) * 16));
         }
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-            const int row = TM + wn + 2 * col + j;
+            const int row = TM + wn + j * 32 + col;
             o.b[j] = *reinterpret_cast<const int4_t*>(buffer + row * BK + (((kk * 2 + half) ^ ((row >> 2) & 3)) * 16));
         }
     };
