@@ -11,6 +11,7 @@
 #include "tensor_ops.hpp"
 
 #include <algorithm>
+#include <cmath>
 
 #include "../../include/fvsrn.h"
 #include "tensor_elements.hpp"
@@ -1205,7 +1206,7 @@ hipError_t withLane(const ScanPlan& plan, F&& f) {
 ScanPlan planScan(const ScanParams& p, int dtype, bool backward) {
     ScanPlan plan{};
     plan.slots = plan.parts = plan.vec = plan.chunks = plan.waves = 1;
-    const long long step = std::llabs(p.xs[1]), next = std::llabs(p.xs[2]) * p.G;
+    const double step = std::fabs(double(p.xs[1])), next = std::fabs(double(p.xs[2])) * p.G;  // (any 64-bit strides)
     // Lanes along the steps where steps lie closer together than gates (colours along a ray: step 4, next ray's far away), or where there are too few
     // gates beside each other: 64 x 4096 steps of 6 channels take 31 us with lanes along the steps and 27 along the channels, backward 54 and 55; 4 channels
     // 19 and 27, 28 and 53; 12 channels 56 and 28, 115 and 58.

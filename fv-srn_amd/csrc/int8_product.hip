@@ -573,11 +573,13 @@ hipError_t withType(int dtype, F&& f) {
 
 }  // namespace
 
+// 16 values of a lane in rows of up to 1024: what a row costs beside its values -- the maximum's way through the lanes, the reciprocal -- is spread over them
+int quantizeWidth(int cols) { return std::min(64, powerOfTwoAtLeast(cols <= 1024 ? (cols + 15) / 16 : (cols + 7) / 8)); }
+
 hipError_t launch_quantize_rows(const QuantizeParams& p, int dtype, hipStream_t s) {
     return withType(dtype, [&](auto element) {
         typedef decltype(element) T;
-        // 16 values of a lane in rows of up to 1024: what a row costs beside its values -- the maximum's way through the lanes, the reciprocal -- is spread over them
-        const int width = std::min(64, powerOfTwoAtLeast(p.cols <= 1024 ? (p.cols + 15) / 16 : (p.cols + 7) / 8));
+        const int width = quantizeWidth(p.cols);
         auto launch = [&](auto held, auto rows) {
             constexpr int H = decltype(held)::value, R = decltype(rows)::value;
             const long long rowsOfBlock = 4 * (64 / width) * R;

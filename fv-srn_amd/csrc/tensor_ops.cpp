@@ -35,12 +35,14 @@ bool rangeOf(const char* name, const void* ptr, size_t element, int dims, const 
     return true;
 }
 
+unsigned long long magnitude(long long v) { return v < 0 ? 0ull - (unsigned long long)v : (unsigned long long)v; }
+
 // Two elements (of `extent` strides' units each) of an output share an address: sorted by stride, some dimension does not step over all of the smaller ones
 bool overlapsItself(const long long* size, const long long* stride, int dims, __int128 extent = 1) {
     for (int d = 0; d < dims; ++d)
         if (size[d] == 0) return false;
     int order[3] = {0, 1, 2};
-    std::sort(order, order + dims, [&](int a, int b) { return std::llabs(stride[a]) < std::llabs(stride[b]); });
+    std::sort(order, order + dims, [&](int a, int b) { return magnitude(stride[a]) < magnitude(stride[b]); });
     __int128 reach = extent - 1;
     for (int j = 0; j < dims; ++j) {
         const int d = order[j];
@@ -74,8 +76,8 @@ std::string overlapping(const std::vector<Range>& outputs, const std::vector<Ran
     return "";
 }
 
-// A launch has at most 2^32 - 1 threads in a dimension
-constexpr long long kMaxThreads = 0xffffffffLL;
+// A launch has less than 2^32 threads in a dimension, whole workgroups of up to 256 (of 512: counted in them)
+constexpr long long kMaxThreads = (1LL << 32) - 256;
 
 struct ScanCall {
     const char* what;
@@ -223,7 +225,7 @@ int fvsrn_quantize_rows(const void* d_x, int dtype, long long rows, int cols, lo
         if (!d_x || !d_codes || !d_scales) return fail(FVSRN_ERR_INVALID_ARGUMENT, "null pointer");
         if ((ldx < cols && !(ldx == 0 || rows == 1)) || (ldc < cols && rows > 1)) return fail(FVSRN_ERR_INVALID_ARGUMENT, "a row stride is smaller than a row");
         if (cols > (1 << 30)) return fail(FVSRN_ERR_UNSUPPORTED, "more than 2^30 columns");
-        if (__int128(rows) * 64 > kMaxThreads) return fail(FVSRN_ERR_UNSUPPORTED, "too many rows for one launch, split the matrix");
+        if (__int128(rows) * quantizeWidth(cols) > kMaxThreads) return fail(FVSRN_ERR_UNSUPPORTED, "too many rows for one launch, split the matrix");
         const long long size[2] = {rows, cols}, sx[2] = {ldx, 1}, sc[2] = {ldc, 1}, one[1] = {1};
         Range x, codes, scales;
         if (!rangeOf("x", d_x, elementSize(dtype), 2, size, sx, x) || !rangeOf("the codes", d_codes, 1, 2, size, sc, codes) || !rangeOf("the scales", d_scales, 4, 1, size, one, scales))
@@ -253,7 +255,8 @@ int fvsrn_matmul_int8(const signed char* d_a, long long lda, const float* d_scal
         if ((lda < K && !(lda == 0 || M == 1)) || (ldb < K && !(ldb == 0 || N == 1)) || (ldo < N && M > 1))
             return fail(FVSRN_ERR_INVALID_ARGUMENT, "a row stride is smaller than a row");
         if (N > (1 << 26)) return fail(FVSRN_ERR_UNSUPPORTED, "too many channels for one launch, split the weights");
-        if (M > (1LL << 31)) return fail(FVSRN_ERR_UNSUPPORTED, "too many rows for one launch, split the matrix");
+        const auto tiles = [&](int edge) { return __int128((M + edge - 1) / edge) * ((N + edge - 1) / edge); };
+        if (M > (1LL << 31) || (M > 64 && N > 16 && (tiles(128) * 256 > kMaxThreads || tiles(256) * 512 > kMaxThreads))) return fail(FVSRN_ERR_UNSUPPORTED, "too many rows for one launch, split the matrix");
         const long long as[2] = {M, K}, bs[2] = {N, K}, os[2] = {M, N}, sa[2] = {lda, 1}, sb[2] = {ldb, 1}, so[2] = {ldo, 1}, one[1] = {1};
         Range a, b, out, scaleA, scaleB, bias;
         if (!rangeOf("a", d_a, 1, 2, as, sa, a) || !rangeOf("b", d_b, 1, 2, bs, sb, b) || !rangeOf("out", d_out, elementSize(out_dtype), 2, os, so, out) ||

@@ -45,6 +45,7 @@ struct QuantizeParams {
     long long rows, ldx, ldc;
     int cols;
 };
+int quantizeWidth(int cols);  // lanes of a row
 hipError_t launch_quantize_rows(const QuantizeParams& p, int dtype, hipStream_t s);
 
 struct Int8Params {

@@ -776,3 +776,33 @@ def test_tensor_refusals():
                  lambda: capi.matmul_int8(f(2, 8, dtype=torch.int8), f(2), f(3, 8, dtype=torch.int8), f(3), dtype=torch.float64)):
         with pytest.raises(capi.FvsrnError):
             call()
+
+
+@no_gpu
+def test_calls_of_more_threads_than_a_launch_has():
+    # (less than 2^32 threads, in whole workgroups; sizes on both sides of the limit)
+    def product(M, N, K=64):
+        return capi.lib().fvsrn_matmul_int8(1 << 20, K, 1 << 50, 1 << 51, K, 1 << 52, None, M, N, K, 5, 1.0, 1 << 53, 1, N, None)
+
+    assert product(1 << 31, 16) == OK  # (256 tokens a workgroup of 256)
+    assert product((1 << 31) - 256, 128) == OK and product((1 << 31) - 255, 128) == -4  # (tiles of 256 tokens and 512 threads)
+    assert product((1 << 31) - 256, 128, 1024) == OK and product((1 << 31) - 255, 17, 1024) == -4
+    assert product((1 << 30) - 128, 129) == OK and product((1 << 30) - 127, 129) == -4  # (tiles of 128 and 256 threads)
+
+    def codes(rows, cols):
+        return capi.lib().fvsrn_quantize_rows(1 << 20, 1, rows, cols, cols, 1 << 50, cols, 1 << 52, None)
+
+    assert codes((1 << 26) - 4, 1024) == OK and codes((1 << 26) - 3, 1024) == -4  # (a wave each)
+    assert codes((1 << 28) - 16, 250) == OK and codes((1 << 28) - 15, 250) == -4  # (16 lanes each)
+    # rows of one step and one gate, a lane each
+    assert scan_call(desc(B=(1 << 31), T=1, Ch=1, Cg=1, gate_stride=(0, 0, 0), x_stride=(0, 0, 0), out_stride=(1, 1, 1)), out=1 << 50, last=1 << 52, h0=None) == OK
+    for B, want in (((1 << 31) - 128, OK), ((1 << 31) - 127, -4)):
+        assert scan_call(desc(B=B, T=1, Ch=2, Cg=2, gate_stride=(0, 0, 0), x_stride=(0, 0, 0), out_stride=(2, 2, 1)), out=1 << 50, last=1 << 52, h0=None) == want
+
+
+@no_gpu
+def test_strides_of_dimensions_of_one_may_be_anything():
+    for s in (-(1 << 63), (1 << 63) - 1):
+        assert scan_call(desc(B=1, T=1, Ch=1, Cg=1, x_stride=(s, s, s), gate_stride=(s, s, s), out_stride=(s, s, s))) == OK
+        assert scan_call(desc(B=1, x_stride=(s, 6, 1), out_stride=(s, 6, 1))) == OK
+        assert scan_call(desc(B=2, out_stride=(s, 6, 1))) == -1
