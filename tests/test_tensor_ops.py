@@ -806,3 +806,82 @@ def test_strides_of_dimensions_of_one_may_be_anything():
         assert scan_call(desc(B=1, T=1, Ch=1, Cg=1, x_stride=(s, s, s), gate_stride=(s, s, s), out_stride=(s, s, s))) == OK
         assert scan_call(desc(B=1, x_stride=(s, 6, 1), out_stride=(s, 6, 1))) == OK
         assert scan_call(desc(B=2, out_stride=(s, 6, 1))) == -1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=["f32", "f16", "bf16"])
+@pytest.mark.parametrize("shape", [(5, 700, 3, 1), (2, 9000, 4, 1), (3, 300, 64, 64), (2, 3000, 70, 70), (2, 300, 260, 2)], ids=lambda s: "x".join(map(str, s)))
+def test_scan_opaque_and_empty_samples(shape, dtype):
+    """Gates of exactly 0 and 1: absorptions of infinity, of the type's largest value and of 0.  The same products and sums as by value, so the same bits."""
+    B, T, Ch, Cg = shape
+    r = np.random.RandomState(5)
+    kind = torch.from_numpy(r.randint(0, 12, (B, T, Cg))).cuda()
+    absorption = torch.zeros(B, T, Cg, device="cuda", dtype=dtype)
+    absorption[kind == 0], absorption[kind == 1] = math.inf, torch.finfo(dtype).max
+    value = (kind > 1).to(dtype)
+    case = scan_inputs(B, T, Ch, Cg, dtype, capi.GATE_VALUE, 6)
+    case["gate"] = value
+    for blend in (capi.INPUT_ADD, capi.INPUT_BLEND):
+        for reverse in (False, True):
+            how = dict(input_mode=blend, reverse=reverse)
+            want = check_scan(case, dict(how, gate_mode=capi.GATE_VALUE, gate_scale=1.0))
+            how |= dict(gate_mode=capi.GATE_EXP, gate_scale=-2.0, h0=case["h0"])
+            out, last = capi.gated_scan(absorption, case["x"], **how)
+            dgate, dx, dh0 = capi.gated_scan_backward(absorption, case["x"], case["dout"], case["dlast"], **how)
+            for name, got in (("out", out), ("last", last), ("dx", dx), ("dh0", dh0)):
+                assert torch.equal(got, want[name]), name
+            assert torch.equal(dgate[value == 0], torch.zeros_like(dgate[value == 0]))
+            # -2 v is exact, but not what is left of a subnormal v: with s the step there (2^-24 of fp16) the rounding of v is off by s / 2, doubled s, and that of
+            # -2 v by s / 2 again, 1.5 s together; both are multiples of s, so they are at most s apart
+            f = torch.finfo(dtype)
+            off = (dgate.double() + 2 * want["dgate"].double()).abs()[value == 1]
+            assert (off <= torch.where(want["dgate"][value == 1].abs() < f.tiny, f.tiny * f.eps, 0.0)).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(40, 300, 2, 2), (2, 9000, 1, 1), (2, 3000, 64, 64), (2, 5000, 70, 70)], ids=lambda s: "x".join(map(str, s)))
+def test_scan_calls_at_once_on_two_streams_and_of_one_tensor(shape):
+    """gate and x may be one tensor; two calls may run beside each other, each with scratch memory of its own."""
+    how = modes(3)
+    cases = [scan_inputs(*shape, F32, how["gate_mode"], s) for s in (1, 2)]
+
+    def both(c):
+        out, last = capi.gated_scan(c["gate"], c["gate"], h0=c["h0"], **how)
+        return (out, last) + capi.gated_scan_backward(c["gate"], c["gate"], c["dout"], c["dlast"], h0=c["h0"], **how)
+
+    want = [both(c) for c in cases]
+    for c, w in zip(cases, want):
+        plain = plain_scan(c["gate"], c["gate"], c["dout"], c["dlast"], h0=c["h0"], **how)
+        for name, got in zip(("out", "last", "dgate", "dx", "dh0"), w):
+            assert_within(got, plain[name], name)
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    got = []
+    for turn in range(4):
+        for s, c in zip(streams, cases):
+            with torch.cuda.stream(s):
+                got.append(both(c))
+    torch.cuda.synchronize()
+    for i, g in enumerate(got):
+        for a, b in zip(g, want[i % 2]):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(40, 300, 3, 1), (2, 9000, 3, 1), (2, 3000, 64, 64), (2, 200, 260, 2), (9, 40, 100, 50)], ids=lambda s: "x".join(map(str, s)))
+def test_scan_gradients_one_at_a_time(shape):
+    """The entry without some of its outputs gives the same bits for the others."""
+    how = modes(5)
+    c = scan_inputs(*shape, F32, how["gate_mode"], 9, lengths=True)
+    want = capi.gated_scan_backward(c["gate"], c["x"], c["dout"], c["dlast"], h0=c["h0"], lengths=c["lengths"], **how)
+    d = desc(*shape, gate_mode=how["gate_mode"], input_mode=how["input_mode"], reverse=int(how["reverse"]), gate_scale=how["gate_scale"])
+    n = C.c_size_t(0)
+    assert capi.lib().fvsrn_gated_scan_workspace(C.byref(d), 1, C.byref(n)) == 0
+    ws = torch.empty(max(n.value, 4), dtype=torch.uint8, device="cuda")
+    for asked in range(1, 8):
+        got = [torch.full_like(w, math.nan) if asked >> i & 1 else None for i, w in enumerate(want)]
+        ptr = [None if g is None else g.data_ptr() for g in got]
+        assert backward_call(d, *(c[k].data_ptr() for k in ("gate", "x", "h0", "lengths", "dout", "dlast")), *ptr, ws=ws.data_ptr(), ws_bytes=n.value) == 0
+        torch.cuda.synchronize()
+        for g, w in zip(got, want):
+            assert g is None or torch.equal(g, w), asked
