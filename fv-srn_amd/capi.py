@@ -746,9 +746,13 @@ def _refuse_device(t, what: str, device: int):
     raise FvsrnError(ERR_WRONG_DEVICE, "%s is on HIP device %d, but the current device is %d" % (what, t.get_device(), device))
 
 
+def _nowhere() -> int:
+    return -1
+
+
 def _operand(t, what: str, device: int, dtype, shape=None) -> int:
     """The address of a tensor of the current device, of the given dtype and shape, whatever its strides."""
-    if not hasattr(t, "get_device") or not t.is_cuda or t.get_device() != device:
+    if getattr(t, "get_device", _nowhere)() != device:  # (-1 of a tensor in host memory)
         _refuse_device(t, what, device)
     if t.dtype != dtype:
         raise FvsrnError(-1, "%s must be %s" % (what, dtype))
@@ -790,11 +794,11 @@ def _raw_stream():
     return getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda device: torch.cuda.current_stream(device).cuda_stream)
 
 
-def _allocated(context, make):
+def _empty(context, like, shape, dtype):
     if context is None:
-        return make()
+        return like.new_empty(shape, dtype=dtype)
     with context:
-        return make()
+        return like.new_empty(shape, dtype=dtype)
 
 
 def quantize_rows(x, codes=None, scales=None, stream: Optional[int] = None):
@@ -808,9 +812,9 @@ def quantize_rows(x, codes=None, scales=None, stream: Optional[int] = None):
     xp = _operand(x, "x", device, x.dtype)
     ldx, (rows, cols) = _row_stride(x, "x"), x.shape
     if codes is None:
-        codes = _allocated(context, lambda: torch.empty((rows, cols), dtype=torch.int8, device=x.device))
+        codes = _empty(context, x, (rows, cols), torch.int8)
     if scales is None:
-        scales = _allocated(context, lambda: torch.empty(rows, dtype=torch.float32, device=x.device))
+        scales = _empty(context, x, rows, torch.float32)
     qp, sp = _operand(codes, "codes", device, torch.int8, x.shape), _dense(scales, "scales", device, torch.float32, (rows,))
     _check(lib().fvsrn_quantize_rows(xp, code, rows, cols, ldx, qp, _row_stride(codes, "codes"), sp, s))
     return codes, scales
@@ -837,7 +841,7 @@ def matmul_int8(a, scale_a, b, scale_b, bias=None, activation: str = "None", act
     if code is None:
         raise FvsrnError(-1, "the output must be float32, float16 or bfloat16")
     if out is None:
-        out = _allocated(context, lambda: torch.empty((M, N), dtype=dtype, device=a.device))
+        out = _empty(context, a, (M, N), dtype)
     op = _operand(out, "out", device, dtype, (M, N))
     _check(lib().fvsrn_matmul_int8(ap, lda, sap, bp, ldb, sbp, biasp, M, N, K, act, activation_param, op, code, _row_stride(out, "out"), s))
     return out
@@ -875,16 +879,16 @@ def gated_scan(gate, x, *, gate_mode: int = GATE_VALUE, gate_scale: float = 1.0,
     gp, xp = _operand(gate, "gate", device, dtype), _operand(x, "x", device, dtype)
     shape = x.shape
     if out is None and states:
-        out = _allocated(context, lambda: torch.empty(shape, dtype=dtype, device=x.device))
+        out = _empty(context, x, shape, dtype)
     op = None if out is None else _operand(out, "out", device, dtype, shape)
     _, ref, bytes_ = _scan_plan(code, gate_mode, gate_scale, input_mode, reverse, gate.shape, shape, gate.stride(), x.stride(), None if out is None else out.stride(), None, None, None)
     ends = (shape[0], shape[2])
     if last is None:
-        last = _allocated(context, lambda: torch.empty(ends, dtype=torch.float32, device=x.device))
+        last = _empty(context, x, ends, torch.float32)
     lp = _dense(last, "last", device, torch.float32, ends)
     hp = None if h0 is None else _dense(h0, "h0", device, torch.float32, ends)
     np_ = None if lengths is None else _dense(lengths, "lengths", device, torch.int32, ends[:1])
-    ws = _allocated(context, lambda: torch.empty(bytes_, dtype=torch.uint8, device=x.device)) if bytes_ else None
+    ws = _empty(context, x, bytes_, torch.uint8) if bytes_ else None
     _check(lib().fvsrn_gated_scan(ref, gp, xp, hp, np_, op, lp, None if ws is None else ws.data_ptr(), bytes_, s))
     return out, last
 
@@ -902,20 +906,20 @@ def gated_scan_backward(gate, x, dout=None, dlast=None, *, gate_mode: int = GATE
     gp, xp = _operand(gate, "gate", device, dtype), _operand(x, "x", device, dtype)
     shape = x.shape
     if dgate is None:
-        dgate = _allocated(context, lambda: torch.empty(gate.shape, dtype=dtype, device=x.device))
+        dgate = _empty(context, x, gate.shape, dtype)
     if dx is None:
-        dx = _allocated(context, lambda: torch.empty(shape, dtype=dtype, device=x.device))
+        dx = _empty(context, x, shape, dtype)
     dp = None if dout is None else _operand(dout, "dout", device, dtype, shape)
     dgp, dxp = _operand(dgate, "dgate", device, dtype, gate.shape), _operand(dx, "dx", device, dtype, shape)
     _, ref, bytes_ = _scan_plan(code, gate_mode, gate_scale, input_mode, reverse, gate.shape, shape, gate.stride(), x.stride(), None, None if dout is None else dout.stride(),
                                 dgate.stride(), dx.stride())
     ends = (shape[0], shape[2])
     if dh0 is None and h0 is not None:
-        dh0 = _allocated(context, lambda: torch.empty(ends, dtype=torch.float32, device=x.device))
+        dh0 = _empty(context, x, ends, torch.float32)
     dlp = None if dlast is None else _dense(dlast, "dlast", device, torch.float32, ends)
     hp = None if h0 is None else _dense(h0, "h0", device, torch.float32, ends)
     np_ = None if lengths is None else _dense(lengths, "lengths", device, torch.int32, ends[:1])
     dhp = None if dh0 is None else _dense(dh0, "dh0", device, torch.float32, ends)
-    ws = _allocated(context, lambda: torch.empty(bytes_, dtype=torch.uint8, device=x.device)) if bytes_ else None
+    ws = _empty(context, x, bytes_, torch.uint8) if bytes_ else None
     _check(lib().fvsrn_gated_scan_backward(ref, gp, xp, hp, np_, dp, dlp, dgp, dxp, dhp, None if ws is None else ws.data_ptr(), bytes_, s))
     return dgate, dx, dh0
