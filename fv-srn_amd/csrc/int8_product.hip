@@ -389,7 +389,8 @@ __global__ __launch_bounds__(256) void matmul_int8_narrow_kernel(const Int8Param
 // lane order, so it is their source that is permuted.  A wave's channels are paired -- column l of its piece j is channel 2 l + j -- so that a lane stores two adjacent
 // outputs and a wave whole 128-byte lines of 16-bit ones; they lie in LDS in the order in which they are read (every second row would meet every second
 // bank twice: half of the LDS cycles).
-//   Measured: 8192 x 4096 x 4096 133 us (2.07 POP/s; the matrix units are busy 69 % of the cycles of a clock that falls to 1.65 GHz under them), 262144 x 256 x 256 43 - 46 us
+//   Measured: 8192 x 4096 x 4096 127 - 138 us by card (2.0 - 2.16 POP/s; the matrix units have 64 of 100 cycles of the CUs, LDS reads and writes as many, at a clock that falls to
+// 1.65 - 1.85 GHz under them; two workgroups of 256 x 128 a CU, which load half as much again: 147 - 153 us against 133), 262144 x 256 x 256 43 - 46 us
 // (201 MB, 4.4 - 4.7 TB/s).
 template <class T, int TM, int TN, int WM, int WN, int RING, bool DIRECT>
 __global__ __launch_bounds__(64 * WM * WN) void matmul_int8_tile_kernel(const Int8Params p, const int activation, const int tilesM, const int tilesN) {
