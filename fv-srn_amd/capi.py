@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes as C
 import functools
+import operator
 import os
 from typing import Optional, Sequence
 
@@ -847,9 +848,15 @@ def matmul_int8(a, scale_a, b, scale_b, bias=None, activation: str = "None", act
     return out
 
 
+def _scan_plan(code, gate_mode, gate_scale, input_mode, reverse, *layout):
+    """The description of a scan and the bytes of scratch memory it needs.  The modes and the scale may be tensors: what is kept goes by the values they have at
+    this call (a tensor's hash is its identity, and it would find the description of the values it had before)."""
+    return _described_scan(code, operator.index(gate_mode), float(gate_scale), operator.index(input_mode), bool(reverse), *layout)
+
+
 @functools.lru_cache(maxsize=512)
-def _scan_plan(code, gate_mode, gate_scale, input_mode, reverse, gate_shape, x_shape, gate_stride, x_stride, out_stride, dout_stride, dgate_stride, dx_stride):
-    """The description of a scan of these shapes and strides (None: that operand is not there) and the bytes of scratch memory it needs."""
+def _described_scan(code, gate_mode, gate_scale, input_mode, reverse, gate_shape, x_shape, gate_stride, x_stride, out_stride, dout_stride, dgate_stride, dx_stride):
+    """_scan_plan of plain values, of these shapes and strides (None: that operand is not there)."""
     if len(gate_shape) != 3 or len(x_shape) != 3 or gate_shape[:2] != x_shape[:2]:
         raise FvsrnError(-1, "gate must be (batch, steps, gate channels) and x (batch, steps, channels)")
     d = ScanDesc(dtype=code, gate_mode=gate_mode, input_mode=input_mode, reverse=int(reverse), gate_scale=gate_scale, length=x_shape[1], batch=x_shape[0],

@@ -885,3 +885,36 @@ def test_scan_gradients_one_at_a_time(shape):
         torch.cuda.synchronize()
         for g, w in zip(got, want):
             assert g is None or torch.equal(g, w), asked
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# what a program keeps and changes between its calls
+# ---------------------------------------------------------------------------------------------------------------------
+
+def described(T=5, gate_mode=capi.GATE_EXP, gate_scale=-1.0, input_mode=capi.INPUT_ADD, reverse=False, B=2, Ch=6, Cg=3):
+    dense = lambda c: (T * c, c, 1)  # noqa: E731
+    return capi._scan_plan(0, gate_mode, gate_scale, input_mode, reverse, (B, T, Cg), (B, T, Ch), dense(Cg), dense(Ch), dense(Ch), None, None, None)[0]
+
+
+@pytest.mark.parametrize("name,field,first,second", [("gate_scale", "gate_scale", -0.5, -2.0), ("reverse", "reverse", False, True), ("gate_mode", "gate_mode", 1, 0), ("input_mode", "input_mode", 0, 1)])
+def test_scan_takes_its_description_by_value(name, field, first, second):
+    """A tensor that holds the scale, a mode or the direction and is changed in place: the next call goes by what it holds then."""
+    v = torch.tensor(first)
+    assert getattr(described(**{name: v}), field) == first
+    v.fill_(second)
+    assert getattr(described(**{name: v}), field) == second
+    assert getattr(described(**{name: first}), field) == first
+
+
+@pytest.mark.gpu
+def test_scan_with_a_scale_that_is_trained():
+    gate, x = torch.rand(4, 50, 1, device="cuda") * 5, torch.rand(4, 50, 3, device="cuda")
+    step = torch.nn.Parameter(torch.tensor(-0.5))
+    for value in (-0.5, -2.0):
+        with torch.no_grad():
+            step.fill_(value)
+            how = dict(gate_mode=capi.GATE_EXP, input_mode=capi.INPUT_BLEND)
+            got, want = (capi.gated_scan(gate, x, gate_scale=s, **how) for s in (step, value))
+            back, back_want = (capi.gated_scan_backward(gate, x, x, gate_scale=s, **how) for s in (step, value))
+        for a, b in zip(got + back[:2], want + back_want[:2]):
+            assert torch.equal(a, b)
