@@ -759,6 +759,8 @@ def _operand(t, what: str, device: int, dtype, shape=None) -> int:
         raise FvsrnError(-1, "%s must be %s" % (what, dtype))
     if shape is not None and t.shape != shape:
         raise FvsrnError(-1, "%s must be of shape %s, not %s" % (what, tuple(shape), tuple(t.shape)))
+    if t.is_neg():  # (the imaginary part of a conjugate: the memory holds the values without their minus)
+        raise FvsrnError(-1, "%s is a view that is negated only when it is read: pass %s.resolve_neg()" % (what, what))
     return t.data_ptr()
 
 

@@ -918,3 +918,33 @@ def test_scan_with_a_scale_that_is_trained():
             back, back_want = (capi.gated_scan_backward(gate, x, x, gate_scale=s, **how) for s in (step, value))
         for a, b in zip(got + back[:2], want + back_want[:2]):
             assert torch.equal(a, b)
+
+
+def negated(t, device="cpu"):
+    """t as the imaginary part of a conjugate: a float32 view of memory that holds -t."""
+    v = torch.complex(torch.zeros_like(t), -t).to(device).conj().imag
+    assert v.is_neg() and torch.equal(v.cpu(), t)
+    return v
+
+
+def test_lazily_negated_views_are_refused():
+    v = negated(torch.randn(2, 5, 3))
+    with pytest.raises(capi.FvsrnError, match="resolve_neg"):
+        capi._operand(v, "x", -1, F32)
+    assert capi._operand(v.resolve_neg(), "x", -1, F32) and capi._operand(v.detach().clone(), "x", -1, F32)
+
+
+@pytest.mark.gpu
+def test_no_operand_may_be_a_lazily_negated_view():
+    t = lambda *s: torch.rand(*s, device="cuda")  # noqa: E731
+    gate, x, h0 = t(2, 5, 3), t(2, 5, 3), t(2, 3)
+    n = lambda v: negated(v.cpu(), "cuda")  # noqa: E731
+    flat = negated(torch.rand(4, 1), "cuda")  # (a matrix of one column has contiguous rows whatever its strides)
+    codes, scales = capi.quantize_rows(flat.resolve_neg())
+    for call in (lambda: capi.gated_scan(n(gate), x), lambda: capi.gated_scan(gate, n(x)), lambda: capi.gated_scan(gate, x, out=n(x)),
+                 lambda: capi.gated_scan(n(gate[:1, :, :1]), x[:1, :, :1], h0=n(h0[:1, :1])), lambda: capi.gated_scan_backward(gate, x, n(x)),
+                 lambda: capi.gated_scan_backward(gate, x, x, dx=n(x)), lambda: capi.gated_scan_backward(gate, x, x, dgate=n(gate)), lambda: capi.quantize_rows(flat),
+                 lambda: capi.matmul_int8(codes, scales, codes, scales, out=n(t(4, 4)))):
+        with pytest.raises(capi.FvsrnError, match="resolve_neg"):
+            call()
+    assert torch.equal(capi.gated_scan(gate, n(x).resolve_neg())[0], capi.gated_scan(gate, x)[0])
