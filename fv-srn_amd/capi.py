@@ -63,7 +63,7 @@ class SceneDesc(C.Structure):
 OPTIONS = {"small_kernel": 0, "persistent": 1, "depth_segments": 2, "fourier_resync": 3, "unit_quota": 4, "tile_order": 5,
            "waves_per_block": 6, "max_blocks_per_cu": 7, "relu_clamp": 8, "keyframe_slots": 9, "working_grids": 10, "overlap_kernel": 11,
            "persistent_reserve": 12, "cell_table": 13}
-ERR_WRONG_DEVICE = -8
+ERR_UNSUPPORTED, ERR_WRONG_DEVICE = -4, -8
 
 GRADIENT_OFF_OR_DIRECT, GRADIENT_FINITE_DIFFERENCES, GRADIENT_ADJOINT_METHOD = 0, 1, 2
 LIGHT_POINT, LIGHT_DIRECTIONAL = 0, 1
@@ -778,6 +778,13 @@ def _row_stride(t, what: str) -> int:
     return t.stride(0)
 
 
+def _int_size(n: int, what: str) -> int:
+    """A size that the C entry takes as an int: ctypes would pass the low 32 bits of a larger one."""
+    if n > 0x7fffffff:
+        raise FvsrnError(ERR_UNSUPPORTED, "%s is over 2^31 - 1" % what)
+    return n
+
+
 def _launch_state(t, what: str, stream):
     """(the current device, the handle of the stream of a call -- `stream` or torch's current one --, a context for its allocations or None where they
     belong to the current stream anyway); t: the first operand, without a device there is nothing to ask"""
@@ -814,6 +821,7 @@ def quantize_rows(x, codes=None, scales=None, stream: Optional[int] = None):
         raise FvsrnError(-1, "x must be float32, float16 or bfloat16")
     xp = _operand(x, "x", device, x.dtype)
     ldx, (rows, cols) = _row_stride(x, "x"), x.shape
+    _int_size(cols, "the number of columns")
     if codes is None:
         codes = _empty(context, x, (rows, cols), torch.int8)
     if scales is None:
@@ -833,6 +841,7 @@ def matmul_int8(a, scale_a, b, scale_b, bias=None, activation: str = "None", act
     (M, K), (N, Kb) = a.shape, b.shape
     if Kb != K:
         raise FvsrnError(-1, "a and b must have rows of the same length")
+    _int_size(N, "the number of channels"), _int_size(K, "the length of a row")
     sap, sbp = _dense(scale_a, "scale_a", device, torch.float32, (M,)), _dense(scale_b, "scale_b", device, torch.float32, (N,))
     biasp = None if bias is None else _dense(bias, "bias", device, torch.float32, (N,))
     act = ACTIVATIONS.get(activation)
@@ -861,7 +870,9 @@ def _described_scan(code, gate_mode, gate_scale, input_mode, reverse, gate_shape
     """_scan_plan of plain values, of these shapes and strides (None: that operand is not there)."""
     if len(gate_shape) != 3 or len(x_shape) != 3 or gate_shape[:2] != x_shape[:2]:
         raise FvsrnError(-1, "gate must be (batch, steps, gate channels) and x (batch, steps, channels)")
-    d = ScanDesc(dtype=code, gate_mode=gate_mode, input_mode=input_mode, reverse=int(reverse), gate_scale=gate_scale, length=x_shape[1], batch=x_shape[0],
+    if not (gate_mode in (GATE_VALUE, GATE_EXP) and input_mode in (INPUT_ADD, INPUT_BLEND)):
+        raise FvsrnError(-1, "unknown gate mode or input mode")
+    d = ScanDesc(dtype=code, gate_mode=gate_mode, input_mode=input_mode, reverse=int(reverse), gate_scale=gate_scale, length=_int_size(x_shape[1], "the number of steps"), batch=x_shape[0],
                  channels=x_shape[2], gate_channels=gate_shape[2])
     for name, stride in (("gate_stride", gate_stride), ("x_stride", x_stride), ("out_stride", out_stride), ("dout_stride", dout_stride),
                          ("dgate_stride", dgate_stride), ("dx_stride", dx_stride)):

@@ -948,3 +948,32 @@ def test_no_operand_may_be_a_lazily_negated_view():
         with pytest.raises(capi.FvsrnError, match="resolve_neg"):
             call()
     assert torch.equal(capi.gated_scan(gate, n(x).resolve_neg())[0], capi.gated_scan(gate, x)[0])
+
+
+def test_sizes_beyond_an_int_are_refused(monkeypatch):
+    """2^32 + n columns, channels or steps are not n of them: tensors without memory (they end at a null pointer where the size passes)."""
+    monkeypatch.setattr(capi, "_launch_state", lambda t, what, stream: (-1, 0, None))
+    meta = lambda *s, dtype=torch.int8: torch.empty(*s, dtype=dtype, device="meta")  # noqa: E731
+    for n in ((1 << 31), (1 << 32) + 64, (1 << 33) + 5):
+        for call in (lambda: capi.quantize_rows(meta(2, n, dtype=F16)), lambda: capi.matmul_int8(meta(1, n), meta(1, dtype=F32), meta(3, n), meta(3, dtype=F32)),
+                     lambda: capi.matmul_int8(meta(1, 64), meta(1, dtype=F32), meta(n, 64), meta(n, dtype=F32)), lambda: described(T=n),
+                     lambda: capi.gated_scan(meta(1, n, 1, dtype=F16), meta(1, n, 1, dtype=F16)), lambda: capi.gated_scan_backward(*[meta(1, n, 1, dtype=F16)] * 3)):
+            with pytest.raises(capi.FvsrnError) as e:
+                call()
+            assert e.value.code == -4, e.value
+    for mode in (dict(gate_mode=1 << 32), dict(input_mode=1 << 32), dict(gate_mode=2), dict(input_mode=-1)):
+        with pytest.raises(capi.FvsrnError):
+            described(**mode)
+
+
+@pytest.mark.gpu
+def test_rows_beyond_an_int_are_refused():
+    """The same with memory behind them: rows of 2^32 + 64 codes, of which 64 would be read."""
+    a = torch.empty(1, (1 << 32) + 64, dtype=torch.int8, device="cuda")
+    one = torch.ones(1, device="cuda")
+    out = torch.full((1, 1), 7.0, device="cuda")
+    with pytest.raises(capi.FvsrnError):
+        capi.matmul_int8(a, one, a, one, out=out)
+    with pytest.raises(capi.FvsrnError):
+        capi.quantize_rows(torch.empty(1, (1 << 32) + 64, dtype=F16, device="cuda"))
+    assert float(out) == 7.0
