@@ -813,7 +813,8 @@ def _empty(context, like, shape, dtype):
 
 def quantize_rows(x, codes=None, scales=None, stream: Optional[int] = None):
     """Codes (rows, cols) int8 and scales (rows,) float32 of the rows of a float32 / float16 / bfloat16 matrix (fvsrn_quantize_rows): scale = max |x| / 127, code =
-    x / scale to the nearest.  Tokens and the (out, in) weights of a layer alike.  A row that holds an infinity or a NaN: scale NaN, codes 0."""
+    x / scale to the nearest.  Tokens and the (out, in) weights of a layer alike.  A row that holds an infinity or a NaN: scale NaN, codes 0.  Codes have no
+    gradient, and neither has what matmul_int8 makes of them."""
     import torch
     device, s, context = _launch_state(x, "x", stream)
     code = _tensor_dtypes().get(getattr(x, "dtype", None))
@@ -886,7 +887,8 @@ def gated_scan(gate, x, *, gate_mode: int = GATE_VALUE, gate_scale: float = 1.0,
                states: bool = True, out=None, last=None, stream: Optional[int] = None):
     """h_t = a_t h_{t-1} + u_t over (batch, steps, channels), a_t = gate or exp(gate_scale * gate), u_t = x or (1 - a_t) x (fvsrn_gated_scan).  gate has (batch,
     steps, gate channels), each for channels / gate channels adjacent channels of x.  Returns (all states -- None with states=False --, the last state (batch,
-    channels) float32).  h0: float32 (batch, channels); lengths: int32 (batch,); last may be h0: a march that steps in place.
+    channels) float32).  h0: float32 (batch, channels); lengths: int32 (batch,); last may be h0: a march that steps in place.  No graph is recorded: where one
+    would be (gate, x or h0 requires a gradient and gradients are enabled) the call is refused, gated_scan_backward has the gradients.
 
     Beer-Lambert blending of the colours (rays, samples, rgb + absorption) that Scene.evaluate_tf gives, back to front:
         _, rgb = gated_scan(c[..., 3:], c[..., :3], gate_mode=GATE_EXP, gate_scale=-stepsize, input_mode=INPUT_BLEND, reverse=True, states=False)"""
@@ -897,6 +899,9 @@ def gated_scan(gate, x, *, gate_mode: int = GATE_VALUE, gate_scale: float = 1.0,
     if code is None:
         raise FvsrnError(-1, "gate must be float32, float16 or bfloat16")
     gp, xp = _operand(gate, "gate", device, dtype), _operand(x, "x", device, dtype)
+    if (gate.requires_grad or x.requires_grad or getattr(h0, "requires_grad", False)) and torch.is_grad_enabled():
+        raise FvsrnError(-1, "gated_scan records no graph, its gradients are those of gated_scan_backward: call both in a torch.autograd.Function, or this one under "
+                             "torch.no_grad() or with detached tensors")
     shape = x.shape
     if out is None and states:
         out = _empty(context, x, shape, dtype)

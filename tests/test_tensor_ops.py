@@ -977,3 +977,45 @@ def test_rows_beyond_an_int_are_refused():
     with pytest.raises(capi.FvsrnError):
         capi.quantize_rows(torch.empty(1, (1 << 32) + 64, dtype=F16, device="cuda"))
     assert float(out) == 7.0
+
+
+def test_scan_does_not_drop_a_gradient(monkeypatch):
+    """Tensors without memory: a call that passes ends at a null pointer."""
+    monkeypatch.setattr(capi, "_launch_state", lambda t, what, stream: (-1, 0, None))
+    meta = lambda *s, grad=False: torch.empty(*s, device="meta").requires_grad_(grad)  # noqa: E731
+    for trained in range(3):
+        gate, x, h0 = (meta(*s, grad=i == trained) for i, s in enumerate(((2, 5, 3), (2, 5, 6), (2, 6))))
+        with pytest.raises(capi.FvsrnError, match="gated_scan_backward"):
+            capi.gated_scan(gate, x, h0=h0)
+        for call in (lambda: capi.gated_scan(gate.detach(), x.detach(), h0=h0.detach()), torch.no_grad()(lambda: capi.gated_scan(gate, x, h0=h0)),
+                     lambda: capi.gated_scan_backward(gate, x, meta(2, 5, 6), h0=h0)):
+            with pytest.raises(capi.FvsrnError, match="null pointer"):
+                call()
+
+
+@pytest.mark.gpu
+def test_scan_in_an_autograd_function():
+    how = modes(7)
+
+    class Blend(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, gate, x, h0):
+            ctx.save_for_backward(gate, x, h0)
+            return capi.gated_scan(gate, x, h0=h0, **how)
+
+        @staticmethod
+        @torch.autograd.function.once_differentiable
+        def backward(ctx, dout, dlast):
+            gate, x, h0 = ctx.saved_tensors
+            return capi.gated_scan_backward(gate, x, dout, dlast, h0=h0, **how)
+
+    for shape in ((5, 60, 3, 1), (2, 300, 64, 64)):
+        c = scan_inputs(*shape, F32, how["gate_mode"], 21)
+        leaves = [c[k].clone().requires_grad_() for k in ("gate", "x", "h0")]
+        out, last = Blend.apply(*leaves)
+        ((out * c["dout"]).sum() + (last * c["dlast"]).sum()).backward()
+        want = plain_scan(c["gate"], c["x"], c["dout"], c["dlast"], h0=c["h0"], **how)
+        for leaf, name in zip(leaves, ("dgate", "dx", "dh0")):
+            assert_within(leaf.grad, want[name], name)
+        with pytest.raises(capi.FvsrnError):
+            capi.gated_scan(*leaves[:2], **how)
