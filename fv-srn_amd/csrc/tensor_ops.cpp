@@ -147,6 +147,7 @@ int fvsrn_gated_scan(const fvsrn_scan_desc* desc, const void* d_gate, const void
         ScanParams& p = c.p;
         if (p.B == 0 || p.C == 0) return FVSRN_OK;
         if (p.T > 0 && (!d_gate || !d_x)) return fail(FVSRN_ERR_INVALID_ARGUMENT, "null pointer");
+        if (p.T == 0 && !d_last) return FVSRN_OK;  // (no states to write; an empty tensor's address may be NULL)
         if (!d_out && !d_last) return fail(FVSRN_ERR_INVALID_ARGUMENT, "neither states nor last states are asked for");
         const size_t e = elementSize(desc->dtype);
         const long long gates[3] = {p.B, p.T, p.Cg}, full[3] = {p.B, p.T, p.C}, ends[2] = {p.B, p.C}, endStride[2] = {p.C, 1}, one[1] = {1};
@@ -184,6 +185,7 @@ int fvsrn_gated_scan_backward(const fvsrn_scan_desc* desc, const void* d_gate, c
         ScanParams& p = c.p;
         if (p.B == 0 || p.C == 0) return FVSRN_OK;
         if (p.T > 0 && (!d_gate || !d_x)) return fail(FVSRN_ERR_INVALID_ARGUMENT, "null pointer");
+        if (p.T == 0 && !d_dh0) return FVSRN_OK;  // (an empty tensor's address may be NULL)
         if (!d_dgate && !d_dx && !d_dh0) return fail(FVSRN_ERR_INVALID_ARGUMENT, "no gradient is asked for");
         const size_t e = elementSize(desc->dtype);
         const long long gates[3] = {p.B, p.T, p.Cg}, full[3] = {p.B, p.T, p.C}, ends[2] = {p.B, p.C}, endStride[2] = {p.C, 1}, one[1] = {1};

@@ -1019,3 +1019,21 @@ def test_scan_in_an_autograd_function():
             assert_within(leaf.grad, want[name], name)
         with pytest.raises(capi.FvsrnError):
             capi.gated_scan(*leaves[:2], **how)
+
+
+@no_gpu
+def test_scans_of_no_steps_that_write_nothing():
+    """Empty tensors have no address: nothing is asked for, and nothing is to be done."""
+    empty = dict(gate=None, x=None, h0=None)
+    assert backward_call(desc(T=0), dout=None, dgate=None, dx=None, dh0=None, **empty) == 0
+    assert scan_call(desc(T=0), out=None, last=None, **empty) == 0
+    assert backward_call(desc(T=0), dout=None, dgate=None, dx=None, **empty) == OK and scan_call(desc(T=0), out=None, **empty) == OK  # (there is something to write)
+    assert backward_call(desc(T=0, dtype=3), dgate=None, dx=None, dh0=None, **empty) == -1
+
+
+@pytest.mark.gpu
+def test_scan_gradients_of_no_steps_without_a_state():
+    for shape in ((3, 0, 8), (2, 0, 3)):
+        gate, x = torch.empty(shape[0], 0, 1, device="cuda"), torch.empty(shape, device="cuda")
+        dgate, dx, dh0 = capi.gated_scan_backward(gate, x, torch.empty(shape, device="cuda"), torch.randn(shape[0], shape[2], device="cuda"))
+        assert dgate.shape == gate.shape and dx.shape == x.shape and dh0 is None
