@@ -269,6 +269,12 @@ __global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW) void scan_channels_kernel(
         loadChannels<T, V, L>(xp, p.xs[1], i, n, inside, p.reverse, rawX);
     };
     load(begin + w * L);
+    // d_last may be d_h0, and wave 0 stores it when it has passed the last tile's barrier: by then every wave's h0 has to be here.  ldsBarrier does not wait for it, so
+    // it is waited for in front of the first one.  (Without a tile there is no barrier, and what wave 0 stores is h0 itself.)
+    if constexpr (NW > 1 && !AGGREGATE) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) asm volatile("" : "+v"(h[v]));
+    }
     for (int tile = begin; tile < end; tile += NW * L) {
         const int i0 = tile + w * L;
         float a[L][GV], u[L][V], a2[GV], u2[V];

@@ -1037,3 +1037,20 @@ def test_scan_gradients_of_no_steps_without_a_state():
         gate, x = torch.empty(shape[0], 0, 1, device="cuda"), torch.empty(shape, device="cuda")
         dgate, dx, dh0 = capi.gated_scan_backward(gate, x, torch.empty(shape, device="cuda"), torch.randn(shape[0], shape[2], device="cuda"))
         assert dgate.shape == gate.shape and dx.shape == x.shape and dh0 is None
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(1, 100, 64, 64), (1, 256, 256, 256), (3, 37, 70, 70), (1, 300, 300, 100), (1, 20000, 2, 1), (40, 300, 3, 1), (2, 500, 128, 128)], ids=lambda s: "x".join(map(str, s)))
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+def test_scan_state_in_place_equals_a_state_apart(shape, dtype):
+    """last = h0 in every layout: eight or sixteen waves on a tile in one launch, spans, rows; sequences that end early, and empty ones."""
+    for i in (3, 6):
+        how = modes(i)
+        c = scan_inputs(*shape, dtype, how["gate_mode"], 31, lengths=True)
+        for lengths in (c["lengths"], None):
+            for states in (True, False):
+                want = capi.gated_scan(c["gate"], c["x"], h0=c["h0"], lengths=lengths, states=states, **how)
+                for _ in range(3):
+                    h = c["h0"].clone()
+                    out, last = capi.gated_scan(c["gate"], c["x"], h0=h, last=h, lengths=lengths, states=states, **how)
+                    assert last is h and torch.equal(h, want[1]) and (not states or torch.equal(out, want[0]))
