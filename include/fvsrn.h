@@ -519,7 +519,8 @@ int fvsrn_matmul_int8(const signed char* d_a, long long lda, const float* d_scal
  * d_lengths (int32 per batch element, clamped to 0 .. length; NULL: all `length`): behind a sequence's length nothing is read, and outputs and
  * gradients there are written as zero.  The state is held in 32 bits whatever the dtype; h0 and last are [batch][channels] floats.
  * Inputs may have any strides, zero and negative ones too (broadcast inputs; their gradients come per element); outputs may not overlap themselves.
- * The strides of an operand that is NULL make no address, but its channel stride takes part in the choice of a kernel (and of the scratch memory): leave it 1. */
+ * The strides of an operand that is NULL make no address, but its channel stride takes part in the choice of a kernel (and of the scratch memory), and its step stride
+ * where x is broadcast along the steps: leave them 1 and 0. */
 typedef enum { FVSRN_GATE_VALUE = 0, FVSRN_GATE_EXP = 1 } fvsrn_gate_mode;
 typedef enum { FVSRN_INPUT_ADD = 0, FVSRN_INPUT_BLEND = 1 } fvsrn_input_mode;
 typedef struct {

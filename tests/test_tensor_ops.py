@@ -1054,3 +1054,38 @@ def test_scan_state_in_place_equals_a_state_apart(shape, dtype):
                     h = c["h0"].clone()
                     out, last = capi.gated_scan(c["gate"], c["x"], h0=h, last=h, lengths=lengths, states=states, **how)
                     assert last is h and torch.equal(h, want[1]) and (not states or torch.equal(out, want[0]))
+
+
+@no_gpu
+def test_scan_of_an_input_that_stands_still_is_laid_out_like_a_dense_one():
+    """x broadcast along the steps says nothing of how the others lie: the scratch memory (and with it the layout) is that of a dense x."""
+    def scratch(B, T, Ch, Cg, backward, **kw):
+        n = C.c_size_t(0)
+        assert capi.lib().fvsrn_gated_scan_workspace(C.byref(desc(B, T, Ch, Cg, **kw)), backward, C.byref(n)) == 0
+        return n.value
+
+    for B, T, Ch, Cg in ((8, 4096, 1024, 1024), (1, 9000, 30, 10), (3, 5000, 64, 32)):
+        for backward in (0, 1):
+            dense = scratch(B, T, Ch, Cg, backward)
+            assert dense > 0 and dense == scratch(B, T, Ch, Cg, backward, x_stride=(Ch, 0, 1)) == scratch(B, T, Ch, Cg, backward, x_stride=(0, 0, 1))
+    # steps innermost: the lanes go along them, whichever operand says so
+    B, T, C_ = 2, 9000, 12
+    turned = (T * C_, 1, T)
+    rows = scratch(B, T, C_, C_, 0, x_stride=turned, out_stride=turned, gate_stride=turned)
+    assert rows == scratch(B, T, C_, C_, 0, x_stride=(C_, 0, 1), out_stride=turned, gate_stride=turned) == scratch(B, T, C_, C_, 0, x_stride=(C_, 0, 1), out_stride=(0, 0, 1), gate_stride=turned)
+    assert rows != scratch(B, T, C_, C_, 0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(3, 70, 12, 12), (2, 700, 64, 64), (2, 3000, 70, 70), (2, 300, 60, 20), (3, 600, 30, 30), (2, 9, 10, 10), (4, 300, 3, 1)], ids=lambda s: "x".join(map(str, s)))
+@pytest.mark.parametrize("dtype", [F32, F16], ids=["f32", "f16"])
+def test_scan_of_an_input_that_stands_still(shape, dtype):
+    B, T, Ch, Cg = shape
+    for i in (2, 7):
+        how = modes(i)
+        c = scan_inputs(B, T, Ch, Cg, dtype, how["gate_mode"], 17, lengths=True)
+        c["x"] = c["x"][:, :1].expand(B, T, Ch)
+        assert c["x"].stride(1) == 0
+        check_scan(c, how)
+        c["x"], c["gate"] = c["x"][:1, :, :1].expand(B, T, Ch), c["gate"][:, :1].expand(B, T, Cg)  # (nothing that is read moves)
+        check_scan(c, how, states=False)
