@@ -515,7 +515,9 @@ int fvsrn_matmul_int8(const signed char* d_a, long long lda, const float* d_scal
  * with t running forwards or (reverse) backwards.  Channel c goes by gate c / (channels / gate_channels).  Beer-Lambert blending of n samples
  * along a ray is EXP with gate = absorption and gate_scale = -stepsize, alpha blending is VALUE with gate = 1 - alpha; both BLEND and reverse
  * (back to front), the pixel is `last`.  Gates may be any numbers; products of gates are formed over spans of a sequence, so gates
- * of a magnitude over 1 can overflow there although the recurrence itself would not.
+ * of a magnitude over 1 can overflow there although the recurrence itself would not.  A product below the smallest 32-bit number is 0: an infinite state (backwards: gradient)
+ * that is taken through such a span is NaN behind it (0 times infinity), where one step after the other would have kept the infinity.  What is not finite
+ * stays not finite, in its own channel and from its step on; with finite states and gradients nothing of this is seen.
  * d_lengths (int32 per batch element, clamped to 0 .. length; NULL: all `length`): behind a sequence's length nothing is read, and outputs and
  * gradients there are written as zero.  The state is held in 32 bits whatever the dtype; h0 and last are [batch][channels] floats.
  * Inputs may have any strides, zero and negative ones too (broadcast inputs; their gradients come per element); outputs may not overlap themselves.

@@ -1089,3 +1089,37 @@ def test_scan_of_an_input_that_stands_still(shape, dtype):
         check_scan(c, how)
         c["x"], c["gate"] = c["x"][:1, :, :1].expand(B, T, Ch), c["gate"][:, :1].expand(B, T, Cg)  # (nothing that is read moves)
         check_scan(c, how, states=False)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(3, 90, 3, 1), (3, 90, 64, 64), (3, 3000, 64, 64), (2, 9000, 2, 2), (2, 9000, 3, 1), (3, 400, 16, 2), (3, 400, 66, 22), (2, 1200, 70, 1)], ids=lambda s: "x".join(map(str, s)))
+@pytest.mark.parametrize("reverse", [False, True])
+def test_scan_infinite_states_and_gradients_stay_not_finite(shape, reverse):
+    """An infinity at one step of one channel: infinite there, not finite from there on (the products of gates behind it fall below the smallest 32-bit number), and
+    everything else keeps its bits.  Gradients the same way, towards the sequence's beginning."""
+    B, T, Ch, Cg = shape
+    r = torch.Generator().manual_seed(13)
+    gate, x, dout = (torch.rand(B, T, Cg, generator=r) * 0.5 + 0.25).cuda(), torch.randn(B, T, Ch, generator=r).cuda(), torch.randn(B, T, Ch, generator=r).cuda()
+    h0, dlast = torch.randn(B, Ch, generator=r).cuda(), torch.randn(B, Ch, generator=r).cuda()
+    how = dict(reverse=reverse, h0=h0)
+    clean, back = capi.gated_scan(gate, x, **how), capi.gated_scan_backward(gate, x, dout, dlast, **how)
+    b, c, g = 1, 1, 1 // (Ch // Cg)
+    for at in (0, 40, T - 1):
+        for value in (math.inf, -math.inf):
+            bad = x.clone()
+            bad[b, at, c] = value
+            out, last = capi.gated_scan(gate, bad, **how)
+            later = slice(None, at + 1) if reverse else slice(at, None)
+            assert out[b, at, c] == value and not out[b, later, c].isfinite().any() and not last[b, c].isfinite()
+            assert not (out[b, later, c] == -value).any()  # (gates are positive)
+            for got, want, where in ((out, clean[0], (b, later, c)), (last, clean[1], (b, c))):
+                got[where] = want[where]
+                assert torch.equal(got, want)
+            bad = dout.clone()
+            bad[b, at, c] = value
+            dgate, dx, dh0 = capi.gated_scan_backward(gate, x, bad, dlast, **how)
+            earlier = slice(at, None) if reverse else slice(None, at + 1)
+            assert dx[b, at, c] == value and not dx[b, earlier, c].isfinite().any() and not dgate[b, earlier, g].isfinite().any() and not dh0[b, c].isfinite()
+            for got, want, where in ((dx, back[1], (b, earlier, c)), (dgate, back[0], (b, earlier, g)), (dh0, back[2], (b, c))):
+                got[where] = want[where]
+                assert torch.equal(got, want)
