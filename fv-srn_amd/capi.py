@@ -812,8 +812,8 @@ def _empty(context, like, shape, dtype):
 
 
 def quantize_rows(x, codes=None, scales=None, stream: Optional[int] = None):
-    """Codes (rows, cols) int8 and scales (rows,) float32 of the rows of a float32 / float16 / bfloat16 matrix (fvsrn_quantize_rows): scale = max |x| / 127, code =
-    x / scale to the nearest.  Tokens and the (out, in) weights of a layer alike.  A row that holds an infinity or a NaN: scale NaN, codes 0.  Codes have no
+    """Codes (rows, cols) int8 and scales (rows,) float32 of the rows of a float32 / float16 / bfloat16 matrix (fvsrn_quantize_rows): scale = max(max |x| f,
+    2^-126) with the float32 f next to 1 / 127, code = x / scale (rounded to float32) to the nearest, ties to even.  Tokens and the (out, in) weights of a layer alike.  A row that holds an infinity or a NaN: scale NaN, codes 0.  Codes have no
     gradient, and neither has what matmul_int8 makes of them."""
     import torch
     device, s, context = _launch_state(x, "x", stream)
