@@ -778,30 +778,32 @@ def _row_stride(t, what: str) -> int:
     return t.stride(0)
 
 
-def _int_size(n: int, what: str) -> int:
-    """A size that the C entry takes as an int: ctypes would pass the low 32 bits of a larger one."""
-    if n > 0x7fffffff:
-        raise FvsrnError(ERR_UNSUPPORTED, "%s is over 2^31 - 1" % what)
-    return n
+_INT_MAX = 0x7fffffff  # the largest size where the C entries take an int: ctypes would pass the low 32 bits of a larger one
+
+
+def _refuse_size(what: str):
+    raise FvsrnError(ERR_UNSUPPORTED, "%s is over 2^31 - 1" % what)
 
 
 def _launch_state(t, what: str, stream):
     """(the current device, the handle of the stream of a call -- `stream` or torch's current one --, a context for its allocations or None where they
     belong to the current stream anyway); t: the first operand, without a device there is nothing to ask"""
-    import torch
     if not getattr(t, "is_cuda", False):
         _refuse_device(t, what, -1)
-    device = torch.cuda.current_device()
-    current = _raw_stream()(device)
+    current_device, current_stream = _current()
+    device = current_device()
+    current = current_stream(device)
     if stream is None or stream == current:
         return device, current, None
+    import torch
     return device, stream, torch.cuda.stream(torch.cuda.ExternalStream(stream))
 
 
 @functools.lru_cache(maxsize=None)
-def _raw_stream():
+def _current():
+    """The functions that say which device, and which stream of it, is the current one."""
     import torch
-    return getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda device: torch.cuda.current_stream(device).cuda_stream)
+    return torch.cuda.current_device, getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda device: torch.cuda.current_stream(device).cuda_stream)
 
 
 def _empty(context, like, shape, dtype):
@@ -813,8 +815,8 @@ def _empty(context, like, shape, dtype):
 
 def quantize_rows(x, codes=None, scales=None, stream: Optional[int] = None):
     """Codes (rows, cols) int8 and scales (rows,) float32 of the rows of a float32 / float16 / bfloat16 matrix (fvsrn_quantize_rows): scale = max(max |x| f,
-    2^-126) with the float32 f next to 1 / 127, code = x / scale (rounded to float32) to the nearest, ties to even.  Tokens and the (out, in) weights of a layer alike.  A row that holds an infinity or a NaN: scale NaN, codes 0.  Codes have no
-    gradient, and neither has what matmul_int8 makes of them."""
+    2^-126) with the float32 f next to 1 / 127, code = x / scale (rounded to float32) to the nearest, ties to even.  Tokens and the (out, in) weights of a layer
+    alike.  A row that holds an infinity or a NaN: scale NaN, codes 0.  Codes have no gradient, and neither has what matmul_int8 makes of them."""
     import torch
     device, s, context = _launch_state(x, "x", stream)
     code = _tensor_dtypes().get(getattr(x, "dtype", None))
@@ -822,13 +824,19 @@ def quantize_rows(x, codes=None, scales=None, stream: Optional[int] = None):
         raise FvsrnError(-1, "x must be float32, float16 or bfloat16")
     xp = _operand(x, "x", device, x.dtype)
     ldx, (rows, cols) = _row_stride(x, "x"), x.shape
-    _int_size(cols, "the number of columns")
+    if cols > _INT_MAX:
+        _refuse_size("the number of columns")
     if codes is None:
         codes = _empty(context, x, (rows, cols), torch.int8)
+        qp, ldc = codes.data_ptr(), cols
+    else:
+        qp, ldc = _operand(codes, "codes", device, torch.int8, x.shape), _row_stride(codes, "codes")
     if scales is None:
         scales = _empty(context, x, rows, torch.float32)
-    qp, sp = _operand(codes, "codes", device, torch.int8, x.shape), _dense(scales, "scales", device, torch.float32, (rows,))
-    _check(lib().fvsrn_quantize_rows(xp, code, rows, cols, ldx, qp, _row_stride(codes, "codes"), sp, s))
+        sp = scales.data_ptr()
+    else:
+        sp = _dense(scales, "scales", device, torch.float32, (rows,))
+    _check(lib().fvsrn_quantize_rows(xp, code, rows, cols, ldx, qp, ldc, sp, s))
     return codes, scales
 
 
@@ -842,7 +850,8 @@ def matmul_int8(a, scale_a, b, scale_b, bias=None, activation: str = "None", act
     (M, K), (N, Kb) = a.shape, b.shape
     if Kb != K:
         raise FvsrnError(-1, "a and b must have rows of the same length")
-    _int_size(N, "the number of channels"), _int_size(K, "the length of a row")
+    if N > _INT_MAX or K > _INT_MAX:
+        _refuse_size("the number of channels or the length of a row")
     sap, sbp = _dense(scale_a, "scale_a", device, torch.float32, (M,)), _dense(scale_b, "scale_b", device, torch.float32, (N,))
     biasp = None if bias is None else _dense(bias, "bias", device, torch.float32, (N,))
     act = ACTIVATIONS.get(activation)
@@ -855,8 +864,10 @@ def matmul_int8(a, scale_a, b, scale_b, bias=None, activation: str = "None", act
         raise FvsrnError(-1, "the output must be float32, float16 or bfloat16")
     if out is None:
         out = _empty(context, a, (M, N), dtype)
-    op = _operand(out, "out", device, dtype, (M, N))
-    _check(lib().fvsrn_matmul_int8(ap, lda, sap, bp, ldb, sbp, biasp, M, N, K, act, activation_param, op, code, _row_stride(out, "out"), s))
+        op, ldo = out.data_ptr(), N
+    else:
+        op, ldo = _operand(out, "out", device, dtype, (M, N)), _row_stride(out, "out")
+    _check(lib().fvsrn_matmul_int8(ap, lda, sap, bp, ldb, sbp, biasp, M, N, K, act, activation_param, op, code, ldo, s))
     return out
 
 
@@ -873,7 +884,9 @@ def _described_scan(code, gate_mode, gate_scale, input_mode, reverse, gate_shape
         raise FvsrnError(-1, "gate must be (batch, steps, gate channels) and x (batch, steps, channels)")
     if not (gate_mode in (GATE_VALUE, GATE_EXP) and input_mode in (INPUT_ADD, INPUT_BLEND)):
         raise FvsrnError(-1, "unknown gate mode or input mode")
-    d = ScanDesc(dtype=code, gate_mode=gate_mode, input_mode=input_mode, reverse=int(reverse), gate_scale=gate_scale, length=_int_size(x_shape[1], "the number of steps"), batch=x_shape[0],
+    if x_shape[1] > _INT_MAX:
+        _refuse_size("the number of steps")
+    d = ScanDesc(dtype=code, gate_mode=gate_mode, input_mode=input_mode, reverse=int(reverse), gate_scale=gate_scale, length=x_shape[1], batch=x_shape[0],
                  channels=x_shape[2], gate_channels=gate_shape[2])
     for name, stride in (("gate_stride", gate_stride), ("x_stride", x_stride), ("out_stride", out_stride), ("dout_stride", dout_stride),
                          ("dgate_stride", dgate_stride), ("dx_stride", dx_stride)):
@@ -903,14 +916,20 @@ def gated_scan(gate, x, *, gate_mode: int = GATE_VALUE, gate_scale: float = 1.0,
         raise FvsrnError(-1, "gated_scan records no graph, its gradients are those of gated_scan_backward: call both in a torch.autograd.Function, or this one under "
                              "torch.no_grad() or with detached tensors")
     shape = x.shape
-    if out is None and states:
+    if out is not None:
+        op = _operand(out, "out", device, dtype, shape)
+    elif states:
         out = _empty(context, x, shape, dtype)
-    op = None if out is None else _operand(out, "out", device, dtype, shape)
+        op = out.data_ptr()
+    else:
+        op = None
     _, ref, bytes_ = _scan_plan(code, gate_mode, gate_scale, input_mode, reverse, gate.shape, shape, gate.stride(), x.stride(), None if out is None else out.stride(), None, None, None)
     ends = (shape[0], shape[2])
     if last is None:
         last = _empty(context, x, ends, torch.float32)
-    lp = _dense(last, "last", device, torch.float32, ends)
+        lp = last.data_ptr()
+    else:
+        lp = _dense(last, "last", device, torch.float32, ends)
     hp = None if h0 is None else _dense(h0, "h0", device, torch.float32, ends)
     np_ = None if lengths is None else _dense(lengths, "lengths", device, torch.int32, ends[:1])
     ws = _empty(context, x, bytes_, torch.uint8) if bytes_ else None
@@ -932,19 +951,28 @@ def gated_scan_backward(gate, x, dout=None, dlast=None, *, gate_mode: int = GATE
     shape = x.shape
     if dgate is None:
         dgate = _empty(context, x, gate.shape, dtype)
+        dgp = dgate.data_ptr()
+    else:
+        dgp = _operand(dgate, "dgate", device, dtype, gate.shape)
     if dx is None:
         dx = _empty(context, x, shape, dtype)
+        dxp = dx.data_ptr()
+    else:
+        dxp = _operand(dx, "dx", device, dtype, shape)
     dp = None if dout is None else _operand(dout, "dout", device, dtype, shape)
-    dgp, dxp = _operand(dgate, "dgate", device, dtype, gate.shape), _operand(dx, "dx", device, dtype, shape)
     _, ref, bytes_ = _scan_plan(code, gate_mode, gate_scale, input_mode, reverse, gate.shape, shape, gate.stride(), x.stride(), None, None if dout is None else dout.stride(),
                                 dgate.stride(), dx.stride())
     ends = (shape[0], shape[2])
-    if dh0 is None and h0 is not None:
+    if dh0 is not None:
+        dhp = _dense(dh0, "dh0", device, torch.float32, ends)
+    elif h0 is not None:
         dh0 = _empty(context, x, ends, torch.float32)
+        dhp = dh0.data_ptr()
+    else:
+        dhp = None
     dlp = None if dlast is None else _dense(dlast, "dlast", device, torch.float32, ends)
     hp = None if h0 is None else _dense(h0, "h0", device, torch.float32, ends)
     np_ = None if lengths is None else _dense(lengths, "lengths", device, torch.int32, ends[:1])
-    dhp = None if dh0 is None else _dense(dh0, "dh0", device, torch.float32, ends)
     ws = _empty(context, x, bytes_, torch.uint8) if bytes_ else None
     _check(lib().fvsrn_gated_scan_backward(ref, gp, xp, hp, np_, dp, dlp, dgp, dxp, dhp, None if ws is None else ws.data_ptr(), bytes_, s))
     return dgate, dx, dh0
