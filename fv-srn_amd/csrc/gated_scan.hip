@@ -217,7 +217,7 @@ __device__ __forceinline__ void foldBehind(const float* wa, const float* wd, lon
 
 // Forward.  AGGREGATE: only (A, U) of this workgroup's span, span 0 with h0 folded in (its A slot then holds h0 for the second launch: d_last may be d_h0).  The second
 // launch takes the spans from the last to the first: what the first launch read last is what the memory-side cache still holds.
-// Measured: 65536 x 1024 bf16 61 us for the spans (268 MB, 4.4 TB/s) and 81 us for the walk (405 MB, 5.0 TB/s); 64 x 512 x 4096 bf16 in one launch 149 us (805 MB,
+// Measured: 65536 x 1024 bf16 61 us for the spans (268 MB, 4.4 TB/s) and 79 us for the walk (405 MB, 5.1 TB/s); 64 x 512 x 4096 bf16 in one launch 149 us (805 MB,
 // 5.4 TB/s).
 template <class T, int NW, int V, bool SHARED, bool AGGREGATE>
 __global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW) void scan_channels_kernel(const ScanParams p, const ScanPlan plan, const int blocks, const long long units) {
@@ -943,8 +943,8 @@ __global__ __launch_bounds__(256) void scan_rows_spans_kernel(const ScanParams p
     }
 }
 
-// Forward: bound by memory where 16-byte pieces come in (262144 rays x 512 with three channels fp32: 435 us, 2.15 GB, 4.95 TB/s), by the gates and the joins in 16 bits (425 us
-// for half the bytes).
+// Forward: bound by memory where 16-byte pieces come in (262144 rays x 512 with three channels fp32: 435 us, 2.15 GB, 4.95 TB/s), by the work on each sample -- its gate,
+// its conversions -- in 16 bits (370 - 425 us for half the bytes; lanes joined by cross-lane moves take 2 % off).
 template <class T, int G>
 __global__ __launch_bounds__(256) void scan_rows_kernel(const ScanParams p, const ScanPlan plan, const bool beside) {
     constexpr int K = kRowSteps;
